@@ -156,6 +156,12 @@ def export_state(sd, arch):
 
 
 def export_config(arch):
+    """``config.json`` of ``arch``."""
+    cfg = _family_config(arch)
+    return dict(cfg, kv_cache_block=arch.kv_cache_block) if arch.kv_cache_block else cfg
+
+
+def _family_config(arch):
     a = arch
     if a.layers is not None:
         layers = []

@@ -32,7 +32,7 @@ from ..layers import RotaryTables, alibi_slopes
 from .feedforward import DenseGLU, SparseGLU, SparseMoE
 from .latent import LatentAttention
 from .mixers import ChannelDelta, DynamicTanh, LayerNorm, TimeMix
-from .state import DecodeGraph, DecodeState, KVRows
+from .state import DecodeGraph, DecodeState, KV8Rows, KVRows
 
 _global_hooks = nn.modules.module._has_any_global_hook
 
@@ -67,6 +67,7 @@ class HFArch:
     norm_head: bool = False               # Baichuan2: rows of lm_head are L2-normalised
     use_logn_attn: bool = False           # Qwen inference-time log-n scaling of queries
     use_cache_quantization: bool = False  # Qwen: keep the decode KV cache in uint8 (per-chunk scale / zero)
+    kv_cache_block: int = 0               # keep the KV cache in 8 bits, with a scale for so many positions of a head (0: in the model's type)
     seq_length: int = 2048                # Qwen: training length for log-n / NTK
     tie_word_embeddings: bool = False
     pad_token_id: Optional[int] = None
@@ -97,7 +98,7 @@ def arch_from_hf_config(cfg: dict, family: Optional[str] = None) -> HFArch:
         return _pafodra_arch(cfg)
     if mt == "megozen":
         return _megozen_arch(cfg)
-    a = HFArch(family=mt)
+    a = HFArch(family=mt, kv_cache_block=int(cfg.get("kv_cache_block", 0)))
     g = cfg.get
     if mt == "qwen":
         a.vocab_size, a.hidden_size = g("vocab_size"), g("hidden_size")
@@ -174,6 +175,8 @@ def _megozen_arch(cfg: dict) -> HFArch:
         window = (l.mixer.get("mask") or {}).get("size")
         if window is not None and window < 1:
             raise ValueError(f"layer {i}: a window of {window} tokens")
+    if cfg.get("kv_cache_block"):
+        raise ValueError("kv_cache_block: latent attention keeps no keys and values of heads")
     return HFArch(family="megozen", vocab_size=cfg["vocab"], hidden_size=cfg["width"], layers=layers,
                   num_hidden_layers=len(layers), num_attention_heads=layers[0].mixer["heads"] if layers else 1,
                   num_key_value_heads=1, norm_eps=cfg["norm"]["eps"], block_norm="layer_norm", expert_form="glu",
@@ -188,8 +191,8 @@ def _pafodra_arch(cfg: dict) -> HFArch:
     return HFArch(family="pafodra", vocab_size=cfg["vocab"], hidden_size=cfg["width"], layers=layers,
                   num_hidden_layers=len(layers), num_attention_heads=att.get("heads", 1),
                   num_key_value_heads=att.get("kv_heads", 1), norm_eps=cfg["norm"]["eps"],
-                  embedding_scale=cfg["embedding"]["scale"], position="none", bos_token_id=cfg.get("bos_token_id"),
-                  eos_token_id=cfg.get("eos_token_id"), pad_token_id=cfg.get("pad_token_id"))
+                  embedding_scale=cfg["embedding"]["scale"], position="none", kv_cache_block=int(cfg.get("kv_cache_block", 0)),
+                  bos_token_id=cfg.get("bos_token_id"), eos_token_id=cfg.get("eos_token_id"), pad_token_id=cfg.get("pad_token_id"))
 
 
 def weight_owner(layers, i):
@@ -249,6 +252,8 @@ class Attention(nn.Module):
         return [[p.weight for p in ps]] + ([[p.bias for p in ps]] if self.a.qkv_bias else [])
 
     def new_state(self, slots, capacity, device, dtype):
+        if self.a.kv_cache_block:
+            return KV8Rows(slots, capacity, self.hk, self.d, self.dv, self.a.kv_cache_block, device)
         if self.a.use_cache_quantization:
             from .kv_quant import QuantizedKV
             return {"kq": QuantizedKV(slots, capacity, self.hk, self.d, device, dtype),
@@ -268,11 +273,15 @@ class Attention(nn.Module):
 
     def _attend(self, q, k, v, meta, cache, appended=False):
         """Serving attention: prompts that start here on the prefill kernel, everything else over the cached rows.
-        ``cache``: the layer's ``KVRows``, or None for packed sequences that keep nothing.  ``appended``: it has the step's keys."""
+        ``cache``: the layer's ``KVRows`` or ``KV8Rows``, or None for packed sequences that keep nothing.  ``appended``: it has the step's
+        keys."""
         T = q.shape[0]
+        eight = isinstance(cache, KV8Rows)
         sl = self.slopes.to(q.device) if self.slopes is not None else None
         sink = self.sink.detach() if self.sink is not None else None
-        if cache is not None and not appended:
+        if eight:
+            iops.kv8_append(cache.cache, k, v, meta)
+        elif cache is not None and not appended:
             iops.kv_append(cache.k, cache.v, k, v, meta)
         fresh = cache is None or (meta["fresh"] and not meta["one_token"])
         if fresh and iops.prefill_kernel_ok(q, v):
@@ -280,6 +289,9 @@ class Attention(nn.Module):
             if row_start is None:
                 row_start = ops.cuda.row_start_of(meta["cu_seqlens"], T, q.device)
             o = iops.attention_prefill(q, k, v, row_start, self.scale, sink, sl)
+        elif eight:
+            o = iops.attention_kv8(q, cache.cache, meta["kv_base"], meta["kv_len"], meta.get("kv_bound", meta["max_position"]), self.scale, sink,
+                                   sl, cu_seqlens=None if meta["one_token"] else meta["cu_seqlens"], max_q=meta["max_seqlen"])
         elif cache is not None:
             o = iops.attention_rows(q, cache.k.view(-1, self.hk, self.d), cache.v.view(-1, self.hk, self.dv),
                                     meta["kv_base"], meta["kv_len"], meta.get("kv_bound", meta["max_position"]),
@@ -324,7 +336,7 @@ class Attention(nn.Module):
         if a.use_logn_attn and not self.training:
             logn = torch.clamp(torch.log(pos.float() + 1) / math.log(a.seq_length), min=1.0)
             q = (q.float() * logn.view(T, 1, 1)).to(q.dtype)
-        if isinstance(cache, KVRows):
+        if isinstance(cache, (KVRows, KV8Rows)):
             o = self._attend(q, k, v, meta, cache, appended)
         elif cache is not None:               # dense batch of equal length in a dict: 8-bit cache, draft trees, prefixes
             B = meta["batch"]
@@ -783,7 +795,7 @@ class CausalLM(nn.Module):
         tokens are appended after column ``s``).  A row ends at ``eos_token_id`` or when its tail equals one of
         ``stop_words_ids`` (token sequences; the stop sequence stays in the output, later positions are filled with eos).
         ``cuda_graph``: on a GPU, replay the decode step as a CUDA graph once it has run eagerly (not with dynamic NTK,
-        whose tables depend on the length, nor with the 8-bit cache).
+        whose tables depend on the length, nor with Qwen's dense 8-bit cache).
         ``soft_prefix``: ``{"embeds": [P, hidden]}`` (prompt tuning: virtual input embeddings in front of the
         prompt) or ``{"kv": [layers, 2, P, kv_heads, head_dim]}`` (prefix tuning: pre-filled cache entries)."""
         from ...infer.generation import sample_next
@@ -814,7 +826,8 @@ class CausalLM(nn.Module):
                     c.load_prefix(slots, k0, v0)
             for i in slots:
                 state.lengths[i] = n_kv
-        if a.use_cache_quantization and (not bool(real.all()) or slots != list(range(b))):
+        dense = a.use_cache_quantization and not a.kv_cache_block
+        if dense and (not bool(real.all()) or slots != list(range(b))):
             raise ValueError("the 8-bit cache holds a dense batch: prompts of one length only")
         embeds = None
         if n_emb:
@@ -834,7 +847,7 @@ class CausalLM(nn.Module):
                 logits = graph.step(toks[:, -1])
             else:
                 logits = self.logits(self.step(state, slots, toks[:, -1])[0])
-                if cuda_graph and dev.type == "cuda" and dt != torch.float16 and not a.use_cache_quantization and \
+                if cuda_graph and dev.type == "cuda" and dt != torch.float16 and not dense and \
                         a.rope_dynamic_ntk_max_pos is None and max_new_tokens - step > 4:
                     graph = DecodeGraph(self, state, slots)
             if repetition_penalty != 1.0:

@@ -6,6 +6,7 @@ layer contributes one state object through ``layer.new_state``:
 
 * ``PositionRows``: something for every position, ``[slots, capacity, ...]``, grown in whole blocks of positions; as
   ``KVRows`` keys and values ``[.., kv_heads, dim]``, as ``LatentRows`` one latent and one rotated key part per position;
+* ``KV8Rows``: keys and values for every position in 8 bits, with a scale for each block of positions and head;
 * ``SlotTensors``: fixed-size tensors per slot (recurrent matrices, last inputs of a short convolution or a token shift);
 * a plain dict (the 8-bit cache of Qwen): dense batches of equal length only.
 
@@ -20,6 +21,7 @@ import numpy as np
 import torch
 
 from ... import ops
+from ...ops import infer as iops
 
 BLOCK = 256          # positions a key/value cache grows by
 
@@ -54,6 +56,29 @@ class KVRows(PositionRows):
         """Fill positions ``0 .. n`` of ``slots`` with given keys / values ``[n, kv_heads, dim]`` (prefix tuning)."""
         for s in slots:
             self.k[s, :k.shape[0]], self.v[s, :v.shape[0]] = k.to(self.k.dtype), v.to(self.v.dtype)
+
+
+class KV8Rows:
+    """Keys and values ``[slots, capacity]`` in 8 bits (``cache``, an ``ops.infer.KV8``); ``block`` positions of a head share a scale."""
+
+    def __init__(self, slots, capacity, kv_heads, dim, vdim, block, device):
+        self.sizes, self.device, self.slots, self.capacity = (kv_heads, dim, vdim, block), device, slots, capacity
+        self.cache = iops.kv8_empty(slots * capacity, *self.sizes, device)
+
+    def grow(self, slots, capacity):
+        new = iops.kv8_empty(slots * capacity, *self.sizes, self.device)
+        for old, t in zip(self.cache[:4], new[:4]):
+            old = old.view(self.slots, -1, *old.shape[1:])
+            t.view(slots, -1, *t.shape[1:])[:self.slots, :old.shape[1]] = old
+        self.cache, self.slots, self.capacity = new, slots, capacity
+
+    def load_prefix(self, slots, k, v):
+        """Fill positions ``0 .. n`` of ``slots`` with given keys / values ``[n, kv_heads, dim]`` (prefix tuning)."""
+        n, dev = k.shape[0], self.device
+        for s in slots:
+            at = torch.full((n,), s * self.capacity, dtype=torch.int32, device=dev)
+            iops.kv8_append(self.cache, k, v, {"kv_base": at, "kv_len": torch.arange(1, n + 1, dtype=torch.int32, device=dev), "max_seqlen": n,
+                                               "cu_seqlens": torch.tensor([0, n], dtype=torch.int32, device=dev)})
 
 
 class SlotTensors:

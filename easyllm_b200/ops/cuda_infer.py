@@ -2,6 +2,7 @@
 and the tcgen05 GEMM / attention) for bf16 and fp32 CUDA tensors; the signatures are those of ``ops.infer``."""
 from __future__ import annotations
 
+from contextlib import nullcontext
 from ctypes import addressof, c_float, c_int, c_longlong
 
 import torch
@@ -275,6 +276,51 @@ def attention_rows(q, k, v, base, length, max_len, scale, sink=None, alibi_slope
                                c_int(_heads(v, "v")), _gate(gate, q)[1], c_int(max_len), c_int(window or 0), c_float(scale),
                                _p(cu_seqlens), c_int(n_seq), c_int(max_q), c_longlong(min(k.shape[0], v.shape[0])), _bf(q.dtype),
                                _p(err_flag(q.device)), _stream()), "attn_rows", 2 if need else 1)
+    return out
+
+
+# ---- a cache held in 8 bits ------------------------------------------------------------------------
+def _kv8(cache):
+    return [_p(t) for t in cache[:4]]
+
+
+def _kv8_sizes(cache):
+    return [c_int(cache.k.shape[1]), c_int(cache.dim), c_int(cache.vdim)], [c_int(cache.block.bit_length() - 1), c_longlong(cache.k.shape[0])]
+
+
+def _on(device):
+    """The context in which ``device`` is the current one."""
+    return nullcontext() if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def kv8_append(cache, k, v, base, length, cu_seqlens, max_new):
+    sizes, place = _kv8_sizes(cache)
+    with _on(k.device):
+        _check(lib().ell_kv8_append(*_kv8(cache), _p(k), _p(v), _p(base), _p(length), _p(cu_seqlens), c_int(k.shape[0]),
+                                    c_int(cu_seqlens.numel() - 1), c_int(max_new), *sizes, c_int(_heads(k, "k")), c_int(_heads(v, "v")), *place,
+                                    _bf(k.dtype), _p(err_flag(k.device)), _stream()), "kv8_append")
+
+
+def kv8_read(cache, base, length, max_len, dtype):
+    n, dev = base.numel(), cache.k.device
+    sizes, place = _kv8_sizes(cache)
+    with _on(dev):
+        out = [torch.empty(n, max_len, cache.k.shape[1], w, dtype=dtype, device=dev) for w in (cache.dim, cache.vdim)]
+        _check(lib().ell_kv8_read(*_kv8(cache), _p(out[0]), _p(out[1]), _p(base), _p(length), c_int(n), c_int(max_len), *sizes, *place, _bf(dtype),
+                                  _p(err_flag(dev)), _stream()), "kv8_read")
+    return out[0], out[1]
+
+
+def attention_kv8(q, cache, base, length, max_len, scale, sink=None, alibi_slopes=None, window=None, cu_seqlens=None, max_q=None):
+    T, H, _ = q.shape
+    n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, max_q)
+    sizes, place = _kv8_sizes(cache)
+    with _on(q.device):
+        out = torch.empty(T, H, cache.vdim, dtype=q.dtype, device=q.device)
+        sl = cu._slopes(alibi_slopes, H, q.device)
+        _check(lib().ell_attn_kv8(_p(q), *_kv8(cache), _p(out), _p(base), _p(length), _p(None if sink is None else _f32(sink, "sink")), _p(sl),
+                                  _p(cu_seqlens), c_int(T), c_int(n_seq), c_int(max_q), c_int(H), *sizes, c_int(_heads(q, "q")), c_int(max_len),
+                                  c_int(window or 0), c_float(scale), *place, _bf(q.dtype), _p(err_flag(q.device)), _stream()), "attn_kv8")
     return out
 
 

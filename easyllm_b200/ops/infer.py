@@ -7,6 +7,8 @@ weight bytes; in fp32 they are true fp32 library products.  ``meta`` is the pack
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 import torch.nn.functional as F
 
@@ -232,6 +234,106 @@ def attention_rows(q, k, v, kv_base, kv_len, max_len, scale, sink=None, alibi_sl
     if _kern(q):
         return _cu().attention_rows(q, k, v, kv_base, kv_len, max_len, scale, sink, alibi_slopes, window, gate, cu_seqlens, max_q)
     return ref.attention_rows(q, k, v, kv_base, kv_len, scale, sink, alibi_slopes, window, gate)
+
+
+# ---- a cache held in 8 bits -------------------------------------------------------------------------
+KV8_MOST = 128          # head sizes, and rows that share a scale
+
+
+class KV8(NamedTuple):
+    """Keys and values of the cache rows of a layer in 8 bits: k ``[R, G, dim]``, v ``[R, G, vdim]`` int8 with head sizes padded to
+    multiples of 16, and for each block of rows and head a scale, k_scale / v_scale ``[R / block, G]`` fp32 (``block``: a power of two up to
+    128).  A value is ``int8 * scale``.  Scales are powers of two, the least of which 127 times is the block's largest magnitude or more (at most 2^121: larger values become 127 times that), so
+    that nothing but the rounding to 8 bits is ever lost: values are exact in bf16 and fp32, and in a block that rows join one by one they
+    are off by less than one scale.  Where a block got a value that is not finite, it reads as NaN."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    dim: int
+    vdim: int
+
+    @property
+    def block(self):
+        return self.k.shape[0] // self.k_scale.shape[0]
+
+
+def kv8_empty(rows, heads, dim, vdim, block, device=None):
+    """A ``KV8`` of ``rows`` rows, a multiple of ``block``."""
+    if not 1 <= min(dim, vdim) <= max(dim, vdim) <= KV8_MOST or block < 1 or block > KV8_MOST or block & (block - 1) or rows % block:
+        raise ValueError(f"an 8-bit cache has heads of up to {KV8_MOST} (got {dim}, {vdim}) and rows in blocks of a power of two up to "
+                         f"{KV8_MOST} (got {rows} in blocks of {block})")
+    q = [torch.zeros(rows, heads, -(-w // 16) * 16, dtype=torch.int8, device=device) for w in (dim, vdim)]
+    return KV8(*q, *(torch.zeros(rows // block, heads, device=device) for _ in q), dim, vdim)
+
+
+def _kv8_check(cache, *ints):
+    k, v, ks, vs, d, dv = cache
+    R, G = k.shape[:2]
+    block = R // max(1, ks.shape[0])
+    if k.shape != (R, G, -(-d // 16) * 16) or v.shape != (R, G, -(-dv // 16) * 16) or k.dtype != torch.int8 or v.dtype != torch.int8 or \
+            not 1 <= min(d, dv) <= max(d, dv) <= KV8_MOST or ks.shape != vs.shape or ks.shape != (R // block if block else 0, G) or \
+            ks.shape[0] * block != R or not 1 <= block <= KV8_MOST or block & (block - 1) or ks.dtype != torch.float32 or vs.dtype != torch.float32 or \
+            not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError("an 8-bit cache is contiguous: int8 [R, G, dim padded to 16] rows, fp32 [R / block, G] scales, blocks of a power of two")
+    for t in (v, ks, vs) + ints:
+        if t.device != k.device:
+            raise ValueError(f"8-bit cache on {k.device}, an operand on {t.device}")
+    for t in ints:
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            raise ValueError("places and lengths of cache rows are contiguous int32 vectors")
+    return block
+
+
+def kv8_append(cache, k, v, meta):
+    """Quantise the step's keys k ``[T, G, dim]`` and values v ``[T, G, vdim]`` into their places of ``cache``: the rows between two borders
+    of ``meta["cu_seqlens"]`` are the next tokens of one sequence, of which the first goes to row ``kv_base + kv_len - 1`` (a sequence starts
+    at a block; the sequences of a step are distinct).  Rows behind the last border, and sequences whose ``kv_len`` is 0, are left out.
+    A block that has rows already keeps the larger scale; if that is the new one, its rows are rounded again."""
+    no_grad_check(k, v)
+    base, length, cu = meta["kv_base"], meta["kv_len"], meta["cu_seqlens"]
+    _kv8_check(cache, base, length, cu)
+    T, G = k.shape[0], cache.k.shape[1]
+    if k.shape != (T, G, cache.dim) or v.shape != (T, G, cache.vdim) or k.dtype != v.dtype or k.device != cache.k.device or v.device != k.device or \
+            base.numel() != T or length.numel() != T:
+        raise ValueError(f"kv8_append: k [T, {G}, {cache.dim}] and v [T, {G}, {cache.vdim}] of one dtype, a place and a length for each row")
+    if _kern(k):
+        return _cu().kv8_append(cache, k, v, base, length, cu, meta["max_seqlen"])
+    ref.kv8_append(cache, k, v, meta)
+
+
+def kv8_read(cache, kv_base, kv_len, max_len, dtype=torch.bfloat16):
+    """The values of ``cache`` as keys ``[n, max_len, G, dim]`` and values ``[n, max_len, G, vdim]``: for each sequence the rows ``kv_base`` ..
+    ``kv_base + kv_len`` (at most ``max_len``), then zeros.  Exact in bf16 and fp32."""
+    _kv8_check(cache, kv_base, kv_len)
+    if kv_base.shape != kv_len.shape or dtype not in (torch.bfloat16, torch.float32) or max_len < 0:
+        raise ValueError("kv8_read: a place and a length for each sequence, into bf16 or fp32")
+    if cache.k.is_cuda:
+        return _cu().kv8_read(cache, kv_base, kv_len, max_len, dtype)
+    return ref.kv8_read(cache, kv_base, kv_len, max_len, dtype)
+
+
+def attention_kv8(q, cache, kv_base, kv_len, max_len, scale, sink=None, alibi_slopes=None, window=None, cu_seqlens=None, max_q=None):
+    """``attention_rows`` over an 8-bit cache: row t of q ``[T, H, dim]`` attends to the cache rows ``kv_base[t]`` .. ``kv_base[t] + kv_len[t]``
+    and sits at the last of them.  ``max_len`` bounds ``kv_len``.  ``cu_seqlens`` (with ``max_q``, a bound of their lengths): the rows between two
+    borders are consecutive tokens of one sequence, so they can share its keys.  Rows with nothing to see (``kv_len`` 0, or behind the last
+    border) are zero."""
+    no_grad_check(q)
+    ints = (kv_base, kv_len) if cu_seqlens is None else (kv_base, kv_len, cu_seqlens)
+    _kv8_check(cache, *ints)
+    T, H, d = q.shape
+    if d != cache.dim or H % cache.k.shape[1] or q.device != cache.k.device or kv_base.numel() != T or kv_len.numel() != T:
+        raise ValueError(f"attention_kv8: q [T, H, {cache.dim}] with a multiple of {cache.k.shape[1]} heads, a place and a length for each row")
+    if window is not None and window < 1:
+        raise ValueError(f"attention_kv8: a window of {window} rows")
+    for t, name in ((sink, "sink"), (alibi_slopes, "alibi_slopes")):
+        if t is not None and t.numel() != H:
+            raise ValueError(f"attention_kv8: {name} has one value for each of the {H} heads, got {t.numel()}")
+    if cu_seqlens is not None and max_q is None:
+        raise ValueError("attention_kv8: cu_seqlens comes with max_q, a bound of the sequences' rows")
+    if _kern(q):
+        return _cu().attention_kv8(q, cache, kv_base, kv_len, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
+    return ref.attention_kv8(q, cache, kv_base, kv_len, scale, sink, alibi_slopes, window, cu_seqlens)
 
 
 def prefill_kernel_ok(q, v):

@@ -106,6 +106,93 @@ def attention_rows(q, k, v, kv_base, kv_len, scale, sink=None, alibi_slopes=None
     return out
 
 
+# ---- a cache held in 8 bits ---------------------------------------------------------------------
+def kv8_scale(amax):
+    """Scale of a block whose largest magnitude is ``amax`` (fp32): the least power of two, 2^-126 or more, of which 127 times is
+    ``amax`` or more, but no more than 2^121 (what lies above 127 times that, a percent below the end of the range, becomes that); NaN
+    where ``amax`` is not finite."""
+    m, e = torch.frexp(amax.float())                               # amax = m 2^e, 1/2 <= m < 1
+    e = torch.where(amax == 0, -126, torch.where(m <= 127 / 128, e - 7, e - 6)).clamp(-126, 121)
+    power = ((e.int() + 127) << 23).view(torch.float32)
+    return torch.where(torch.isfinite(amax), power, float("nan"))
+
+
+def kv8_append(cache, k, v, meta):
+    """The step's rows k ``[T, G, d]``, v ``[T, G, dv]`` into their places of ``cache``, see ``infer.kv8_append``."""
+    cu, base, length = (meta[n].tolist() for n in ("cu_seqlens", "kv_base", "kv_len"))
+    B = cache.block
+    for r0, r1 in zip(cu[:-1], cu[1:]):
+        r1 = min(r1, k.shape[0])
+        if r1 <= r0 or length[r0] < 1:
+            continue
+        kv8_place(cache, base[r0], length[r0] - 1 + r1 - r0)
+        for q, scale, x in ((cache.k, cache.k_scale, k[r0:r1].float()), (cache.v, cache.v_scale, v[r0:r1].float())):
+            at, end, row = base[r0] + length[r0] - 1, base[r0] + length[r0] - 1 + r1 - r0, base[r0] + length[r0] - 1
+            while at < end:
+                b, stop = at // B, min((at // B + 1) * B, end)
+                y = x[at - row:stop - row]
+                s = kv8_scale(y.abs().amax((0, 2)))
+                if at > b * B:                                     # rows that were there take the scale that serves both
+                    old = scale[b].clone()
+                    s = torch.maximum(old, s)
+                    q[b * B:at] = torch.nan_to_num(torch.round(q[b * B:at].float() * (old / s).view(1, -1, 1))).to(torch.int8)
+                scale[b] = s
+                q[at:stop] = 0
+                q[at:stop, :, :x.shape[2]] = torch.nan_to_num(torch.round(y / s.view(1, -1, 1)), 0.0, 0.0, 0.0).clamp(-127, 127).to(torch.int8)
+                at = stop
+
+
+def kv8_place(cache, base, n):
+    if base < 0 or base % cache.block or base + n > cache.k.shape[0]:
+        raise ValueError(f"rows {base} .. {base + n} are not in the 8-bit cache of {cache.k.shape[0]}, from the start of a block of {cache.block}")
+
+
+def kv8_rows(cache, first, n):
+    """fp32 keys ``[n, G, dim]`` and values ``[n, G, vdim]`` of the rows from ``first`` on."""
+    at = torch.arange(first, first + n, device=cache.k.device)
+    return [q[at][..., :w].float() * scale[at // cache.block].unsqueeze(-1)
+            for q, scale, w in ((cache.k, cache.k_scale, cache.dim), (cache.v, cache.v_scale, cache.vdim))]
+
+
+def kv8_read(cache, kv_base, kv_len, max_len, dtype):
+    out = [torch.zeros(kv_base.numel(), max_len, cache.k.shape[1], w, dtype=dtype, device=cache.k.device) for w in (cache.dim, cache.vdim)]
+    for i, (base, n) in enumerate(zip(kv_base.tolist(), kv_len.tolist())):
+        n = min(n, max_len)
+        if n > 0:
+            kv8_place(cache, base, n)
+            for o, x in zip(out, kv8_rows(cache, base, n)):
+                o[i, :n] = x.to(dtype)
+    return out[0], out[1]
+
+
+def attention_kv8(q, cache, kv_base, kv_len, scale, sink=None, alibi_slopes=None, window=None, cu_seqlens=None):
+    """``attention_rows`` over the values that the cache stands for; a row that sees nothing is zero."""
+    T, H = q.shape[0] if cu_seqlens is None else min(q.shape[0], int(cu_seqlens[-1])), q.shape[1]
+    G, base, length = cache.k.shape[1], kv_base.tolist(), kv_len.tolist()
+    out = torch.zeros(q.shape[0], H, cache.vdim, dtype=q.dtype, device=q.device)
+    t = 0
+    while t < T:
+        e = t + 1
+        while e < T and base[e] == base[t] and length[e] == length[e - 1] + 1:
+            e += 1
+        n = length[e - 1]
+        if n > 0:
+            kv8_place(cache, base[t], n)
+            ks, vs = (x.repeat_interleave(H // G, 1) for x in kv8_rows(cache, base[t], n))
+        for r in range(t, e):                                      # rows it does not see are not touched: they may hold anything
+            lo, hi = max(0, length[r] - window) if window else 0, length[r]
+            if hi <= 0:
+                continue
+            s = torch.einsum("hd,khd->hk", q[r].float(), ks[lo:hi]) * scale
+            if alibi_slopes is not None:
+                s = s + alibi_slopes.float().view(-1, 1) * (torch.arange(lo, hi, device=q.device) - (hi - 1))
+            if sink is not None:
+                s = torch.cat((s, sink.float().view(H, 1)), -1)
+            out[r] = torch.einsum("hk,khd->hd", torch.softmax(s, -1)[:, :hi - lo], vs[lo:hi]).to(q.dtype)
+        t = e
+    return out
+
+
 def token_mix(h, mu, cu, slots, pos0, tail):
     """``h + (h_prev - h) * mu_c`` for every row of ``mu [C, W]`` → ``[C, T, W]``; ``tail [slots, W]`` carries the
     last row of every sequence."""
