@@ -598,6 +598,20 @@ int make_tmap_bf16_heads(CUtensorMap* map, const void* ptr, uint64_t dim, uint64
   return r == CUDA_SUCCESS ? 0 : -12;
 }
 
+// Packed rows of bytes [rows, heads, dim] in boxes of one head, `box_rows` rows and 128 bytes (columns past `dim` read as zero).
+int make_tmap_bytes_heads(CUtensorMap* map, const void* ptr, uint64_t dim, uint64_t heads, uint64_t rows, uint32_t box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return -10;
+  if ((reinterpret_cast<uintptr_t>(ptr) & 15) || (dim & 15)) return -11;
+  cuuint64_t dims[3] = {dim, heads, rows};
+  cuuint64_t strides[2] = {dim, dim * heads};
+  cuuint32_t box[3] = {128, 1, box_rows};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -12;
+}
+
 template <int BN, bool A_MN, bool B_MN, int OUT, bool HAS_BIAS, int FUSE = kFuseNone>
 static int launch_gemm(const CUtensorMap& tA, const CUtensorMap& tB, const CUtensorMap& tC, const FuseArgs& fuse,
                        const __nv_bfloat16* bias, int M, int N, int K, int ldc, int* err, int max_ctas,

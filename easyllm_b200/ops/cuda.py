@@ -39,7 +39,7 @@ def lib():
             raise KernelError(f"{_LIB_PATH} is missing: run `python -m easyllm_b200.ops.build` "
                               "(or __graft_entry__.build()) before using the CUDA ops")
         _lib = ctypes.CDLL(_LIB_PATH if os.path.exists(_LIB_PATH) else _SERVE_LIB_PATH)
-        for name in ("ell_rmsnorm_bwd_scratch_elems", "ell_attn_rows_scratch", "ell_attn_latent_scratch",
+        for name in ("ell_rmsnorm_bwd_scratch_elems", "ell_attn_rows_scratch", "ell_attn_latent_scratch", "ell_attn_kv8_scratch",
                      "ell_scan_chunks_work", "ell_decoder_step_work", "ell_decoder_layer_kept", "ell_decoder_layer_work"):
             if hasattr(_lib, name):            # the library of the serving kernels has no training step
                 getattr(_lib, name).restype = c_longlong
@@ -103,7 +103,7 @@ def check_err_flag():
                           "17 its work items; 14 latent attention over cached rows, 18 attention over cached rows; 21-24 the attention's "
                           "backward pass, 21 also the cross-entropy exchange; "
                           "31 a token id outside the embedding table; 32 a position outside the rotary tables; "
-                          "41 a scan over chunks; 51 a sequence outside an 8-bit cache, or one that starts inside a block of it; "
+                          "41 a scan over chunks; 51 a sequence outside an 8-bit cache, or one that starts inside a block of it, 52 attention over one; "
                           "6 / 16 a tile index outside a fused kernel's buffers)")
 
 
