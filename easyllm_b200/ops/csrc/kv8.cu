@@ -135,92 +135,144 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Cache c, T* __re
 // ---- attention -----------------------------------------------------------------------------------
 // All products are integer products of the tensor cores (mma.sync m16n8k32), of the cache's bytes as they are: nothing is converted on
 // the way, 23 bytes a clock and SM at the memory's rate.  A query row becomes integers of 23 bits, in units of 2^-21 of its largest
-// element's power of two, a weight times its value's scale integers of 23 bits of the largest of 32 of them; each is cut into three bytes,
+// element's power of two, a weight times its value's scale integers of 23 bits of the largest of 64 of them; each is cut into three bytes,
 // which are rows of the left operand, and the three 32-bit sums, exact, join in fp32.  So scores and sums are as good as fp32 ones.
 //   rows    groups of 8 (token, head): row r of the operand is the low byte of row r, row r + 8 its middle byte; the high bytes take a
 //           second product, whose upper half is empty or another group's
 //   keys    lane (g = lane / 4, c = lane % 4) holds bytes 32 c .. 32 c + 31 of key g of 8: the columns may come in any order, the queries' do so too
-//   values  the same lane holds columns 16 g .. 16 g + 15 of the keys 8 j + 2 c, 8 j + 2 c + 1 (j < 4), which are those whose scores it has: weights
+//   values  the same lane holds columns 16 g .. 16 g + 15 of the keys 8 j + 2 c, 8 j + 2 c + 1 (j < 8), which are those whose scores it has: weights
 //           need no exchange, and four keys' bytes of a column come together by byte permutations
 //   rings   rows of 128 bytes with TMA's 128-byte swizzle: neither access meets a bank conflict
-// The sums start at 12582912 = 1.5 2^23 taken as bits: a sum below 2^22 read as a float is then 12582912 + sum, and a subtraction converts it.
-constexpr int kK8Threads = 128, kK8Keys = 32, kK8Stage = 2 * kK8Keys * 128, kK8Stages = 3, kK8Ring = 4 * kK8Stages * kK8Stage;
-constexpr int kK8Smem = kK8Ring + 1024;                 // two CTAs an SM, in a split of 196 KB
-constexpr int kK8Heads = 16, kK8MaxSplits = 64;
+constexpr int kK8Threads = 128, kK8Keys = 64, kK8Stage = kK8Keys * 128;       // a stage: keys, or values
+// Stages of a warp and CTAs an SM, which are to fit a split of 196 KB with the system's 1 KB each (112 bytes more take 228 KB, which later
+// kernels find their L1 cut down by).
+template <int NB>
+struct K8Ring {
+  static constexpr int kStages = NB == 1 ? 2 : 3, kCtas = NB == 1 ? 3 : 2, kBytes = 4 * kStages * kK8Stage;
+  uint64_t full[4][kStages];
+  int gave_up, free_stage[4];
+  int piece[4];                   // of the current piece: first token, rows, where it begins, quanta behind its end
+  // A warp's sums of a piece go through one stage, [row][column], largest scores and sums of weights behind them or here.
+  static constexpr int kRows = 8 * NB, kSumBytes = kRows * kK8Dim * 4;
+  static constexpr bool kStatHere = kSumBytes + kRows * 8 > kK8Stage;
+  float2 stat[kStatHere ? 4 * kRows : 1];
+};
+template <int NB>
+constexpr int k8_smem() { return K8Ring<NB>::kBytes + (int)sizeof(K8Ring<NB>); }
+template <int NB>
+constexpr bool k8_fits() { return K8Ring<NB>::kSumBytes <= kK8Stage && K8Ring<NB>::kCtas * (k8_smem<NB>() + 1024) <= 196 * 1024; }
+static_assert(k8_fits<1>() && k8_fits<2>(), "");
+// Place of columns 4 i .. 4 i + 3 of row m: the lanes that write a row's or several rows' columns together meet in no bank.
+__device__ __forceinline__ int k8_sum_at(int m, int i) { return m * kK8Dim + 4 * (i ^ (((m & 7) ^ (2 * (i >> 3))) & 7)); }
+constexpr int kK8Heads = 16;
 constexpr int kK8Wait = 52;                             // error word: a copy did not arrive
 constexpr float kLog2e = 1.4426950408889634f;
-static_assert(2 * (kK8Smem + 1024) <= 196 * 1024, "");
 
 struct Kv8Attn {
   Kv8Cache c;
   const void* q;
   void* out;                      // [n, H, dv]
-  float* part;                    // [n, H, splits, dv + 2] when splits > 1
+  float* part;                    // when shares are cut: two slots a CTA, then the CTAs' K8Cut
   const int *base, *len, *cu;
   const float *sink, *slopes;
-  int n, H, ldq, n_seq, tiles, tt, splits, range, window;
+  int n, H, ldq, n_seq, tiles, tt, cut, window;
   float scale;                    // of the scores, times log2 e 2^-21
   int* err;
 };
+__host__ __device__ __forceinline__ int k8_groups(int H, int G) { return G * ((H / G + kK8Heads - 1) / kK8Heads); }
 
-// The tokens, heads and keys of a CTA: blockIdx.x tile of `tt` tokens of a sequence (cu null: one token each), y: key head and group
-// of its query heads, z: range of keys.
+// Work is counted in quanta of 256 keys, one unit of 64 for each warp of a CTA.  An item is a tile of `tt` tokens of a sequence (cu null: one
+// token) with the query heads of a key head, at most 16 of them.
+constexpr int kK8Quantum = 4 * kK8Keys;
 struct K8Tile {
-  int r0, r1, g, h0, nh, rows, k0, k1, len0, last_first, base;
-  __device__ __forceinline__ bool init(const Kv8Attn& a) {
+  int r0, r1, base, len0, len1, low;              // low: where its keys begin, at a unit
+  __device__ __forceinline__ K8Tile(const Kv8Attn& a, int x) {
+    r0 = x;
+    r1 = x + 1;
     if (a.cu != nullptr) {
-      const int seq = blockIdx.x / a.tiles, end = min(a.cu[seq + 1], a.n);
-      r0 = a.cu[seq] + blockIdx.x % a.tiles * a.tt;
+      const int seq = x / a.tiles, end = min(a.cu[seq + 1], a.n);
+      r0 = a.cu[seq] + x % a.tiles * a.tt;
       r1 = min(r0 + a.tt, end);
-    } else {
-      r0 = blockIdx.x;
-      r1 = r0 + 1;
     }
-    const int rep = a.H / a.c.G, groups = (rep + kK8Heads - 1) / kK8Heads;
-    g = blockIdx.y / groups;
-    h0 = g * rep + blockIdx.y % groups * kK8Heads;
-    nh = min(kK8Heads, (g + 1) * rep - h0);
-    if (r0 >= r1) return false;
-    rows = (r1 - r0) * nh;
-    base = a.base[r0];
+    len0 = len1 = low = base = 0;
+    if (r0 >= r1) return;
     len0 = a.len[r0];
-    const int len1 = a.len[r1 - 1];
-    k0 = k1 = 0;
-    last_first = max(0, len1 - a.window);
-    if (len1 > 0) {
-      if (!k8_inside(a.c, base, len1)) {
-        if (threadIdx.x == 0) atomicCAS(a.err, 0, kK8Place);
-      } else {
-        k0 = (max(0, len0 - a.window) & ~(kK8Keys - 1)) + (int)blockIdx.z * a.range;
-        k1 = min(k0 + a.range, len1);
-      }
+    len1 = a.len[r1 - 1];
+    base = a.base[r0];
+    if (len1 > 0 && !k8_inside(a.c, base, len1)) {
+      atomicCAS(a.err, 0, kK8Place);
+      len0 = len1 = 0;
     }
-    return true;
+    low = max(0, len0 - a.window) & ~(kK8Keys - 1);
   }
-  __device__ __forceinline__ int token(int m) const { return r0 + m / nh; }
-  __device__ __forceinline__ int head(int m) const { return h0 + m % nh; }
+  __device__ __forceinline__ int quanta() const { return r0 >= r1 ? 0 : max(1, (len1 - low + kK8Quantum - 1) / kK8Quantum); }
 };
+// What a CTA does at a time: quanta q0 .. q1 - 1 of a tile.
+struct K8Piece {
+  K8Tile t;
+  int q0, q1, quanta;
+  __device__ __forceinline__ K8Piece(const Kv8Attn& a, int x, int q0_, int most) : t(a, x), q0(q0_) {
+    quanta = t.quanta();
+    q1 = min(quanta, q0 + most);
+  }
+  __device__ __forceinline__ int k0() const { return t.low + q0 * kK8Quantum; }
+  __device__ __forceinline__ int k1() const { return min(t.low + q1 * kK8Quantum, t.len1); }
+  __device__ __forceinline__ int units(int warp) const { return max(0, (k1() - k0() - warp * kK8Keys + kK8Quantum - 1) / kK8Quantum); }
+};
+// The next tile with rows, or n_x.
+__device__ __forceinline__ int k8_next(const Kv8Attn& a, int n_x, int x) {
+  while (++x < n_x)
+    if (a.cu == nullptr || a.cu[x / a.tiles] + x % a.tiles * a.tt < min(a.cu[x / a.tiles + 1], a.n)) break;
+  return x;
+}
+// What the joining kernel needs to know of an item that begins in a CTA's share and is cut by its end.
+struct K8Cut {
+  int r0, rows, h0, nh, more;     // more: shares after this one that have a piece of it (0: nothing was cut)
+};
+constexpr int kK8SlotRow = kK8Dim + 4;            // floats of a row in a slot: sums | largest score, sum of weights
 
+// Columns 4 lane .. 4 lane + 3 of a head's output.
 template <typename T>
-__device__ __forceinline__ void k8_zero_rows(const Kv8Attn& a, int t0, int h0, int nh) {      // the heads of tokens t0 and on
-  T* out = reinterpret_cast<T*>(a.out);
-  const long long per = (long long)nh * a.c.dv;
-  for (long long i = threadIdx.x; i < (long long)(a.n - t0) * per; i += blockDim.x)
-    out[((size_t)(t0 + i / per) * a.H + h0) * a.c.dv + i % per] = from_f<T>(0.f);
+__device__ __forceinline__ void k8_store_row(const Kv8Attn& a, int tok, int h, int lane, float4 o) {
+  T* out = reinterpret_cast<T*>(a.out) + ((size_t)tok * a.H + h) * a.c.dv + 4 * lane;
+  const float f[4] = {o.x, o.y, o.z, o.w};
+  if (a.c.dv % 4 == 0) {
+    if (4 * lane < a.c.dv) store_v<4>(out, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * lane + i < a.c.dv) out[i] = from_f<T>(f[i]);
+  }
 }
 
-__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-constexpr int kMagic = 0x4b400000;
+// The sums start at 12582912 = 1.5 2^23 taken as bits: a sum below 2^22 read as a float is then 12582912 + sum, and a subtraction converts it.
+constexpr uint32_t kMagic = 0x4b400000;
 constexpr float kMagicF = 12582912.f;
-// The left operand unsigned, a sum that starts here.
-__device__ __forceinline__ void mma_u8_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-               : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kMagic));
+// The left operand signed (queries) or not (weights).  `first`: a sum that starts here, from `zero`.
+template <bool SIGNED>
+__device__ __forceinline__ void mma_i8(int (&c)[4], bool first, const uint32_t (&zero)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+#define ELL_MMA(TYPE)                                                                                                                              \
+  if (first)                                                                                                                                       \
+    asm("mma.sync.aligned.m16n8k32.row.col.s32." TYPE ".s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"       \
+                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])                                                                                  \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(zero[0]), "r"(zero[1]), "r"(zero[2]), "r"(zero[3]));                                                             \
+  else                                                                                                                                             \
+    asm("mma.sync.aligned.m16n8k32.row.col.s32." TYPE ".s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"           \
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])                                                                                  \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  if (SIGNED) {
+    ELL_MMA("s8")
+  } else {
+    ELL_MMA("u8")
+  }
+#undef ELL_MMA
+}
+// A constant that the compiler takes for a variable, so that it is kept in a register instead of made again wherever it is used: an
+// operand of four registers is then put together once.
+__device__ __forceinline__ uint32_t k8_kept(uint32_t x) {
+  uint32_t y;
+  asm volatile("shfl.sync.idx.b32 %0, %1, 0, 31, 0xffffffff;" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ float2 k8_sum(int x, int y) { return sm100::fadd2(make_float2(__int_as_float(x), __int_as_float(y)), make_float2(-kMagicF, -kMagicF)); }
 // high 2^16 + middle 2^8 + low of two sums
@@ -233,6 +285,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // Bytes of 4 x 4: x[i] byte j -> x[j] byte i.
 __device__ __forceinline__ void transpose_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&y)[4]) {
   const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362), cd0 = __byte_perm(c, d, 0x5140), cd1 = __byte_perm(c, d, 0x7362);
@@ -240,20 +297,6 @@ __device__ __forceinline__ void transpose_bytes(uint32_t a, uint32_t b, uint32_t
   y[1] = __byte_perm(ab0, cd0, 0x7632);
   y[2] = __byte_perm(ab1, cd1, 0x5410);
   y[3] = __byte_perm(ab1, cd1, 0x7632);
-}
-
-struct K8Ring {
-  uint64_t full[4][kK8Stages];    // of a warp's stages
-  int gave_up;
-};
-static_assert(sizeof(K8Ring) <= 128, "");
-// The stages start at a multiple of 1024; the barriers lie in what is left in front of them, or behind.
-__device__ __forceinline__ uint8_t* k8_stages(uint8_t* raw) {
-  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-}
-__device__ __forceinline__ K8Ring& k8_ring(uint8_t* raw) {
-  uint8_t* stages = k8_stages(raw);
-  return *reinterpret_cast<K8Ring*>(stages - raw >= 128 ? raw : stages + kK8Ring);
 }
 
 // The 32 elements 32 c .. 32 c + 31 of a row of `d`.
@@ -276,14 +319,13 @@ __device__ __forceinline__ void k8_load_query(const T* src, int c, int d, bool v
 
 // What a warp keeps of a group of 8 rows; lane (g, c) has row g.
 struct K8Rows {
-  uint32_t q[3][4][2];            // bytes of the query: [low, middle, high][32 columns][half]
+  uint32_t q[4][4], high[4][2];   // bytes of the query, of 32 columns each: low and middle as an operand, high
   float size;                     // power of two of its largest element (NaN where it is not finite)
   float m, l, slope;              // largest score (in powers of two), this lane's share of the sum of the weights
   int first, end;                 // keys the row sees
 };
 template <typename T>
-__device__ __forceinline__ void k8_load_rows(const Kv8Attn& a, const K8Tile& t, int m, int c, K8Rows& r) {
-  const int row = min(m, t.rows - 1), tok = t.token(row), h = t.head(row);      // rows past the end repeat the last
+__device__ __forceinline__ void k8_load_rows(const Kv8Attn& a, int tok, int h, int c, K8Rows& r) {
   const T* src = reinterpret_cast<const T*>(a.q) + (size_t)tok * a.ldq + (size_t)h * a.c.d;
   const bool vec = a.c.d % 8 == 0 && (reinterpret_cast<uintptr_t>(src) & (8 * sizeof(T) > 16 ? 15 : 8 * sizeof(T) - 1)) == 0;
   float f[32], big = 0.f;
@@ -295,21 +337,18 @@ __device__ __forceinline__ void k8_load_rows(const Kv8Attn& a, const K8Tile& t, 
   const int e = max((int)(__float_as_uint(big) >> 23), 1);            // biased exponent
   r.size = e >= 255 ? k8_nan() : __uint_as_float((uint32_t)e << 23);
   const float inv = e >= 254 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)(254 - e) << 23);      // 2^-(e - 127)
+  // v + 0x808080 has the three signed digits of v in its bytes, plus 128 each
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      uint32_t p[3] = {0, 0, 0};
+      uint32_t v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int v = __float2int_rn(f[8 * s + 4 * x + i] * inv * 2097152.f);
-        const int lo = (int8_t)v, v1 = (v - lo) >> 8, mid = (int8_t)v1, hi = (v1 - mid) >> 8;
-        p[0] |= (uint32_t)(lo & 255) << (8 * i);
-        p[1] |= (uint32_t)(mid & 255) << (8 * i);
-        p[2] |= (uint32_t)(hi & 255) << (8 * i);
-      }
-#pragma unroll
-      for (int y = 0; y < 3; ++y) r.q[y][s][x] = p[y];
+      for (int i = 0; i < 4; ++i) v[i] = (__float_as_uint(fmaf(f[8 * s + 4 * x + i] * inv, 2097152.f, kMagicF)) - kMagic + 0x808080u) ^ 0x808080u;
+      const uint32_t ab = __byte_perm(v[0], v[1], 0x5140), cd = __byte_perm(v[2], v[3], 0x5140);
+      r.q[s][2 * x] = __byte_perm(ab, cd, 0x5410);
+      r.q[s][2 * x + 1] = __byte_perm(ab, cd, 0x7632);
+      r.high[s][x] = __byte_perm(__byte_perm(v[0], v[1], 0x0062), __byte_perm(v[2], v[3], 0x0062), 0x5410);
     }
   r.end = a.len[tok];
   r.first = max(0, r.end - a.window);
@@ -318,78 +357,97 @@ __device__ __forceinline__ void k8_load_rows(const Kv8Attn& a, const K8Tile& t, 
   r.l = 0.f;
 }
 
-// Scales of the keys 8 j + 2 c + e (index 2 j + e) from those of key `lane` a lane.
-__device__ __forceinline__ void k8_scales(float mine, int shift, int c, float (&s)[8]) {
-  if (shift >= 3) {
+// Scales of the keys 8 j + 2 c + e (index 2 j + e) from those of keys `lane` and lane + 32 a lane.
+__device__ __forceinline__ void k8_scales(const float (&mine)[2], int shift, int c, float (&s)[16]) {
+  if (shift >= 4) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[2 * j] = s[2 * j + 1] = __shfl_sync(0xffffffffu, mine, 8 * j);
+    for (int j = 0; j < 4; ++j) s[4 * j] = s[4 * j + 1] = s[4 * j + 2] = s[4 * j + 3] = __shfl_sync(0xffffffffu, mine[j >> 1], 16 * (j & 1));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = __shfl_sync(0xffffffffu, mine, 8 * (i >> 1) + 2 * c + (i & 1));
+    for (int i = 0; i < 16; ++i) s[i] = __shfl_sync(0xffffffffu, mine[i >> 3], 8 * ((i >> 1) & 3) + 2 * c + (i & 1));
   }
 }
 
-// A group's weights of 32 keys: from scores (integers joined) to bytes.  Returns the factors of the sums before and of these keys'.
+// A group's weights of 64 keys: from scores (integers joined) to bytes.  With the factors of the sums before and of these keys'.
 struct K8Weights {
-  uint32_t p[3][2];               // bytes: [low, middle, high][keys 0 .. 3, 4 .. 7 of the lane]
+  uint32_t p[2][4], high[2][2];   // bytes, of 32 keys each: low and middle as an operand, high
   float before, now;
 };
-__device__ __forceinline__ void k8_softmax(const Kv8Attn& a, K8Rows& r, float (&s)[8], const float (&ks)[8], const float (&vs)[8], int key0, int c, bool mask,
+__device__ __forceinline__ void k8_softmax(const Kv8Attn& a, K8Rows& r, float (&s)[16], const float (&ks)[16], const float (&vs)[16], int key0, int c, bool mask,
                                            K8Weights& w) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) s[i] = s[i] * a.scale * (ks[i] * r.size);
-  bool sees[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) sees[i] = true;
+  for (int i = 0; i < 16; i += 2) {
+    const float2 f = sm100::fmul2(make_float2(ks[i], ks[i + 1]), make_float2(r.size, r.size));
+    const float2 z = sm100::fmul2(sm100::fmul2(make_float2(s[i], s[i + 1]), make_float2(a.scale, a.scale)), f);
+    s[i] = z.x;
+    s[i + 1] = z.y;
+  }
+  uint32_t hidden = 0;
   if (a.slopes != nullptr || mask) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 16; ++i) {
       const int key = key0 + 8 * (i >> 1) + 2 * c + (i & 1);
       s[i] = fmaf(r.slope, (float)(key - (r.end - 1)), s[i]);
-      sees[i] = key >= r.first && key < r.end;
-      if (!sees[i]) s[i] = -INFINITY;
+      if (key < r.first || key >= r.end) {
+        s[i] = -INFINITY;
+        hidden |= 1u << i;
+      }
     }
   }
-  float mx = sm100::fmax3(sm100::fmax3(s[0], s[1], s[2]), sm100::fmax3(s[3], s[4], s[5]), fmaxf(s[6], s[7]));
+  float mx = fmaxf(s[0], s[1]);
+#pragma unroll
+  for (int i = 2; i < 16; i += 2) mx = sm100::fmax3(mx, s[i], s[i + 1]);
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
   const float now = fmaxf(r.m, mx), ref = now == -INFINITY ? 0.f : now;
   w.before = now == -INFINITY ? 1.f : exp2f(r.m - now);                // no key yet: nothing to rescale
   r.m = now;
-  float big = 0.f, sum = 0.f;
+  float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float p = exp2f(s[i] - ref);
-    sum += p;
-    s[i] = sees[i] ? p * vs[i] : 0.f;                                  // what a row does not see may have any scale
-    big = max_nan(big, s[i]);
+  for (int i = 0; i < 16; i += 2) {
+    float2 z = sm100::fadd2(make_float2(s[i], s[i + 1]), make_float2(-ref, -ref));
+    z = make_float2(exp2f(z.x), exp2f(z.y));
+    sum = sm100::fadd2(sum, z);
+    z = sm100::fmul2(z, make_float2(vs[i], vs[i + 1]));
+    s[i] = z.x;
+    s[i + 1] = z.y;
   }
-  r.l = fmaf(r.l, w.before, sum);
+  r.l = fmaf(r.l, w.before, sum.x + sum.y);
+  if (mask) {                                                          // what a row does not see may have any scale
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (hidden >> i & 1) s[i] = 0.f;
+  }
+  float big = max_nan(s[0], s[1]);
+#pragma unroll
+  for (int i = 2; i < 16; i += 2) big = max3_nan(big, s[i], s[i + 1]);
   big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 1));
   big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 2));
   const int e = max((int)(__float_as_uint(big) >> 23), 23);            // weights below 2^-104, of values of 10^-32, lose bits
   const float up = __uint_as_float((uint32_t)(276 - min(e, 254)) << 23);                // big up is in 2^22 .. 2^23
   w.now = big != big ? k8_nan() : __uint_as_float((uint32_t)(e - 22) << 23);
-  uint32_t f[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = __float_as_uint(fmaf(s[i], up, 8388608.f));        // the mantissa is the integer
+  for (int x = 0; x < 4; ++x) {
+    uint32_t f[4];
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const uint32_t ab = __byte_perm(f[4 * x], f[4 * x + 1], 0x5140), cd = __byte_perm(f[4 * x + 2], f[4 * x + 3], 0x5140);
-    const uint32_t ah = __byte_perm(f[4 * x], f[4 * x + 1], 0x0062), ch = __byte_perm(f[4 * x + 2], f[4 * x + 3], 0x0062);
-    w.p[0][x] = __byte_perm(ab, cd, 0x5410);
-    w.p[1][x] = __byte_perm(ab, cd, 0x7632);
-    w.p[2][x] = __byte_perm(ah, ch, 0x5410);
+    for (int i = 0; i < 4; i += 2) {                                   // the mantissa is the integer
+      const float2 z = sm100::ffma2(make_float2(s[4 * x + i], s[4 * x + i + 1]), make_float2(up, up), make_float2(8388608.f, 8388608.f));
+      f[i] = __float_as_uint(z.x);
+      f[i + 1] = __float_as_uint(z.y);
+    }
+    const uint32_t ab = __byte_perm(f[0], f[1], 0x5140), cd = __byte_perm(f[2], f[3], 0x5140);
+    const uint32_t ah = __byte_perm(f[0], f[1], 0x0062), ch = __byte_perm(f[2], f[3], 0x0062);
+    w.p[x >> 1][2 * (x & 1)] = __byte_perm(ab, cd, 0x5410);
+    w.p[x >> 1][2 * (x & 1) + 1] = __byte_perm(ab, cd, 0x7632);
+    w.high[x >> 1][x & 1] = __byte_perm(ah, ch, 0x5410);
   }
 }
 
-// Scores and weighted values of 32 keys, from `key0` on, in a stage of the ring.  acc: columns 32 c + x and 32 c + 16 + x.
+// Scores of 64 keys in a stage of the ring, as joined integers.
 template <int NB>
-__device__ __forceinline__ void k8_unit(const Kv8Attn& a, const uint8_t* stage, int key0, bool mask, const float (&ks)[8], const float (&vs)[8], K8Rows (&r)[NB],
-                                        float2 (&acc)[NB][16], int gr, int c) {
-  float s[NB][8];
+__device__ __forceinline__ void k8_scores(const uint8_t* stage, const K8Rows (&r)[NB], const uint32_t (&high)[4][4], const uint32_t (&zero)[4], float (&s)[NB][16], int gr, int c) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 8; ++j) {
     uint32_t k[8];
     const uint8_t* row = stage + (8 * j + gr) * 128;                   // row & 7 = gr
     const uint4 x = *reinterpret_cast<const uint4*>(row + (((2 * c) ^ gr) << 4)), y = *reinterpret_cast<const uint4*>(row + (((2 * c + 1) ^ gr) << 4));
@@ -397,15 +455,9 @@ __device__ __forceinline__ void k8_unit(const Kv8Attn& a, const uint8_t* stage, 
     int lm[NB][4], hi[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      hi[i] = kMagic;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) lm[b][i] = kMagic;
-    }
-#pragma unroll
-    for (int x4 = 0; x4 < 4; ++x4) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b) mma_s8(lm[b], r[b].q[0][x4][0], r[b].q[1][x4][0], r[b].q[0][x4][1], r[b].q[1][x4][1], k[2 * x4], k[2 * x4 + 1]);
-      mma_s8(hi, r[0].q[2][x4][0], NB == 2 ? r[NB - 1].q[2][x4][0] : 0u, r[0].q[2][x4][1], NB == 2 ? r[NB - 1].q[2][x4][1] : 0u, k[2 * x4], k[2 * x4 + 1]);
+      for (int b = 0; b < NB; ++b) mma_i8<true>(lm[b], i == 0, zero, r[b].q[i], k[2 * i], k[2 * i + 1]);
+      mma_i8<true>(hi, i == 0, zero, high[i], k[2 * i], k[2 * i + 1]);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -414,48 +466,61 @@ __device__ __forceinline__ void k8_unit(const Kv8Attn& a, const uint8_t* stage, 
       s[b][2 * j + 1] = z.y;
     }
   }
-  K8Weights w[NB];
+}
+
+// Adds 64 keys' weighted values.  A lane reads columns 16 g + 8 (half ^ (g >> 1 & 1)) .. of its keys at a time, so that no two lanes meet
+// in a bank; acc[8 half + x] are columns 32 c + 8 (half ^ (c & 1)) + x and that + 16.
+template <int NB>
+__device__ __forceinline__ void k8_values(const uint8_t* stage, const K8Weights (&w)[NB], const uint32_t (&high)[2][4], const uint32_t (&zero)[4], float2 (&acc)[NB][16], int gr, int c) {
 #pragma unroll
-  for (int b = 0; b < NB; ++b) k8_softmax(a, r[b], s[b], ks, vs, key0, c, mask, w[b]);
-  uint4 v[8];                                                          // 16 columns of this lane's 8 keys
+  for (int half = 0; half < 2; ++half) {
+    uint2 v[16];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int key = 8 * (i >> 1) + 2 * c + (i & 1);
-    v[i] = *reinterpret_cast<const uint4*>(stage + kK8Keys * 128 + key * 128 + ((gr ^ (2 * c + (i & 1))) << 4));
-  }
+    for (int i = 0; i < 16; ++i) {
+      const int key = 8 * (i >> 1) + 2 * c + (i & 1);
+      v[i] = *reinterpret_cast<const uint2*>(stage + key * 128 + ((gr ^ (2 * c + (i & 1))) << 4) + 8 * (half ^ (gr >> 1 & 1)));
+    }
 #pragma unroll
-  for (int y = 0; y < 4; ++y) {
-    uint32_t b0[4], b1[4], t[8];
+    for (int y = 0; y < 2; ++y) {
+      uint32_t t[4][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = y == 0 ? v[i].x : y == 1 ? v[i].y : y == 2 ? v[i].z : v[i].w;
-    transpose_bytes(t[0], t[1], t[2], t[3], b0);
-    transpose_bytes(t[4], t[5], t[6], t[7], b1);
+      for (int z = 0; z < 4; ++z)
+        y == 0 ? transpose_bytes(v[4 * z].x, v[4 * z + 1].x, v[4 * z + 2].x, v[4 * z + 3].x, t[z])
+               : transpose_bytes(v[4 * z].y, v[4 * z + 1].y, v[4 * z + 2].y, v[4 * z + 3].y, t[z]);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      int lm[NB][4], hi[4];
+      for (int x = 0; x < 4; ++x) {
+        int lm[NB][4], hi[4];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) mma_u8_first(lm[b], w[b].p[0][0], w[b].p[1][0], w[b].p[0][1], w[b].p[1][1], b0[x], b1[x]);
-      mma_u8_first(hi, w[0].p[2][0], NB == 2 ? w[NB - 1].p[2][0] : 0u, w[0].p[2][1], NB == 2 ? w[NB - 1].p[2][1] : 0u, b0[x], b1[x]);
+        for (int z = 0; z < 2; ++z) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const float2 z = k8_join(lm[b][0], lm[b][1], lm[b][2], lm[b][3], hi[2 * b], hi[2 * b + 1]);
-        float2& o = acc[b][4 * y + x];
-        o = sm100::ffma2(o, make_float2(w[b].before, w[b].before), make_float2(z.x * w[b].now, z.y * w[b].now));
+          for (int b = 0; b < NB; ++b) mma_i8<false>(lm[b], z == 0, zero, w[b].p[z], t[2 * z][x], t[2 * z + 1][x]);
+          mma_i8<false>(hi, z == 0, zero, high[z], t[2 * z][x], t[2 * z + 1][x]);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const float2 z = k8_join(lm[b][0], lm[b][1], lm[b][2], lm[b][3], hi[2 * b], hi[2 * b + 1]);
+          float2& o = acc[b][8 * half + 4 * y + x];
+          o = sm100::ffma2(o, make_float2(w[b].before, w[b].before), sm100::fmul2(z, make_float2(w[b].now, w[b].now)));
+        }
       }
     }
   }
 }
 
-// Few rows: up to 8 NB of them, the keys dealt out to the warps.  A CTA has 4 warps with rings of their own.
+// Few rows: up to 8 NB of them in an item, whose keys are dealt out to four warps with rings of their own.  With `cut` the quanta of all tiles,
+// one after the other, are dealt out in equal shares, and a CTA takes a share for one group of heads, so that none has more to do than another
+// whatever the lengths; an item that goes over the end of a share goes on in the next, and attn_kv8_join_kernel adds its pieces up.  Without, an
+// item a CTA.  The heads of a share are neighbours among the CTAs: they read the same rows at the same time, 128 bytes each (with shares of
+// all items, heads one after the other, memory delivered 555 MB for 423, and 24 sequences of up to 4096 keys with 32 heads took 140 us).
 template <typename T, int NB>
-__global__ void __launch_bounds__(kK8Threads, 2)
+__global__ void __launch_bounds__(kK8Threads, K8Ring<NB>::kCtas)
 attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Kv8Attn a) {
-  extern __shared__ __align__(128) uint8_t k8sm_raw[];
-  uint8_t* sm = k8_stages(k8sm_raw);
-  K8Ring& ring = k8_ring(k8sm_raw);
+  extern __shared__ __align__(1024) uint8_t sm[];
+  constexpr int kStages = K8Ring<NB>::kStages, R = 8 * NB, LD = kK8SlotRow;
+  K8Ring<NB>& ring = *reinterpret_cast<K8Ring<NB>*>(sm + K8Ring<NB>::kBytes);
   if (threadIdx.x == 0) {
     for (int w = 0; w < 4; ++w)
-      for (int i = 0; i < kK8Stages; ++i) sm100::mbar_init(&ring.full[w][i], 1);
+      for (int i = 0; i < kStages; ++i) sm100::mbar_init(&ring.full[w][i], 1);
     sm100::fence_barrier_init();
     sm100::tma_prefetch_desc(&tmK);
     sm100::tma_prefetch_desc(&tmV);
@@ -463,183 +528,326 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   }
   __syncthreads();
   chain_enter();
-  K8Tile t;
-  const bool some = t.init(a);
-  if (a.cu != nullptr && blockIdx.x == gridDim.x - 1 && a.splits == 1) k8_zero_rows<T>(a, min(max(a.cu[a.n_seq], 0), a.n), t.h0, t.nh);
-  if (!some) return;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, gr = lane >> 2, c = lane & 3;
-  uint8_t* stages = sm + warp * kK8Stage * kK8Stages;
-  const int units = t.k1 > t.k0 ? (t.k1 - t.k0 + kK8Keys - 1) / kK8Keys : 0, mine = units > warp ? (units - warp + 3) / 4 : 0;
+  const int n_x = a.cu != nullptr ? a.n_seq * a.tiles : a.n, hs = k8_groups(a.H, a.c.G), rep = a.H / a.c.G, groups = hs / a.c.G;
+  if (a.cu != nullptr && blockIdx.x == 0) {            // rows behind the last sequence
+    T* out = reinterpret_cast<T*>(a.out);
+    const long long per = (long long)a.H * a.c.dv;
+    for (long long i = min(max(a.cu[a.n_seq], 0), a.n) * per + threadIdx.x; i < a.n * per; i += kK8Threads) out[i] = from_f<T>(0.f);
+  }
+  const int hg = blockIdx.x % hs, share = blockIdx.x / hs, g = hg / groups, h0 = g * rep + hg % groups * kK8Heads, nh = min(kK8Heads, (g + 1) * rep - h0);
+  int x = share, q0 = 0, left = 0x7fffffff, all = 0, shares = 1;
+  if (a.cut) {
+    // where the share begins: a thread counts the quanta of its tiles, and walks them if it is there
+    int* found = reinterpret_cast<int*>(sm);           // sums of the warps | tile, quanta before the share's first in it
+    const int chunk = (n_x + kK8Threads - 1) / kK8Threads, first = min((int)threadIdx.x * chunk, n_x), last = min(first + chunk, n_x);
+    int mine = 0;
+    for (int i = first; i < last; ++i) mine += K8Tile(a, i).quanta();
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += y;
+    }
+    if (lane == 31) found[warp] = before;
+    before -= mine;
+    __syncthreads();
+    int total = 0;
+    for (int w = 0; w < 4; ++w) {
+      if (w == warp) before += total;
+      total += found[w];
+    }
+    all = total;
+    shares = max(1, min((int)gridDim.x / hs, total));  // none is empty
+    const int begin = (int)((long long)share * total / shares);
+    left = share < shares ? (int)((share + 1ll) * total / shares) - begin : 0;
+    if (left > 0 && begin >= before && begin < before + mine) {
+      int at = begin - before, i = first;
+      for (; i < last - 1; ++i) {
+        const int q = K8Tile(a, i).quanta();
+        if (at < q) break;
+        at -= q;
+      }
+      found[4] = i;
+      found[5] = at;
+    }
+    if (threadIdx.x == 0) reinterpret_cast<K8Cut*>(a.part + (size_t)gridDim.x * 2 * R * LD)[blockIdx.x].more = 0;
+    __syncthreads();
+    if (left == 0) return;
+    x = found[4];
+    q0 = found[5];
+    sm100::fence_proxy_async_smem();
+    __syncthreads();
+  }
+  uint8_t* stages = sm + warp * kK8Stage * kStages;
   volatile int* gave_up = &ring.gave_up;
-  auto load = [&](int i) {                             // rows past the range are whatever lies there: they are not seen
-    if (i < mine && lane == 0) {
-      uint8_t* st = stages + i % kK8Stages * kK8Stage;
-      uint64_t* bar = &ring.full[warp][i % kK8Stages];
-      const int row = t.base + t.k0 + (warp + 4 * i) * kK8Keys;
-      sm100::mbar_expect_tx(bar, kK8Stage);
-      sm100::tma_load_3d(st, &tmK, bar, 0, t.g, row);
-      sm100::tma_load_3d(st + kK8Keys * 128, &tmV, bar, 0, t.g, row);
+  // Copies run ahead of the arithmetic by up to a ring, into the next piece too, but for one stage, which the sums of a piece go through.
+  int taken = 0, sent = 0;                             // stages waited for, and stages that copies were sent to
+  int s_row, s_left, n_row = 0, n_units = 0;           // the copies' next row, and stages left in their piece; the next piece's
+  auto send = [&](int ahead) {                         // until `ahead` stages are on their way
+    while (sent - taken < ahead) {
+      if (s_left == 0) {
+        if (n_units == 0) return;
+        s_row = n_row;
+        s_left = 2 * n_units;
+        n_units = 0;
+      }
+      if (lane == 0) {                                 // rows past the range are whatever lies there: they are not seen
+        uint64_t* bar = &ring.full[warp][sent % kStages];
+        sm100::mbar_expect_tx(bar, kK8Stage);
+        sm100::tma_load_3d(stages + sent % kStages * kK8Stage, s_left & 1 ? &tmV : &tmK, bar, 0, g, s_row);
+      }
+      if (s_left & 1) s_row += kK8Quantum;
+      --s_left;
+      ++sent;
     }
   };
-  float kn[2], vn[2];                                  // scales of key `lane` of the next two units
-  auto load_scales = [&](int i, float& k, float& v) {
-    if (i < mine) {
-      const size_t at = (size_t)((t.base + min(t.k0 + (warp + 4 * i) * kK8Keys + lane, t.k1 - 1)) >> a.c.shift) * a.c.G + t.g;
-      k = a.c.ks[at];
-      v = a.c.vs[at];
-    }
-  };
+  uint32_t none[4], zero[4];
 #pragma unroll
-  for (int i = 0; i < kK8Stages - 1; ++i) load(i);
-  load_scales(0, kn[0], vn[0]);
-  load_scales(1, kn[1], vn[1]);
-  K8Rows r[NB];
-  float2 acc[NB][16];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    k8_load_rows<T>(a, t, b * 8 + gr, c, r[b]);
-#pragma unroll
-    for (int x = 0; x < 16; ++x) acc[b][x] = make_float2(0.f, 0.f);
+  for (int i = 0; i < 4; ++i) {
+    zero[i] = k8_kept(kMagic);
+    none[i] = k8_kept(0);
   }
-  bool failed = false;
-  for (int i = 0; i < mine; ++i) {
-    float ks[8], vs[8];
-    k8_scales(kn[0], a.c.shift, c, ks);
-    k8_scales(vn[0], a.c.shift, c, vs);
-    kn[0] = kn[1];
-    vn[0] = vn[1];
-    load_scales(i + 2, kn[1], vn[1]);
-    const int stage = i % kK8Stages, key0 = t.k0 + (warp + 4 * i) * kK8Keys;
-    failed = !sm100::mbar_wait_warp(&ring.full[warp][stage], (i / kK8Stages) & 1, gave_up);
-    if (failed) break;
-    load(i + kK8Stages - 1);                           // over the unit before, which all lanes are done with (the fence and the votes)
-    k8_unit<NB>(a, stages + stage * kK8Stage, key0, key0 + kK8Keys > min(t.len0, t.k1) || key0 < t.last_first, ks, vs, r, acc, gr, c);
-    sm100::fence_proxy_async_smem();                   // these reads before the copies that go over them
-    __syncwarp();
-  }
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    r[b].l += __shfl_xor_sync(0xffffffffu, r[b].l, 1);
-    r[b].l += __shfl_xor_sync(0xffffffffu, r[b].l, 2);
-  }
-  if (failed) *gave_up = 1;
-  __syncthreads();
-  if (*gave_up) {                                      // copies in flight land before the CTA ends
+  bool failed = false, fresh = true;
+  while (true) {
+    const K8Piece p(a, x, q0, left);
+    if (p.quanta == 0) return;                         // an item without rows (the shares have none)
     if (threadIdx.x == 0) {
-      atomicCAS(a.err, 0, kK8Wait);
-      const unsigned long long t0 = sm100::globaltimer_ns();
-      while (sm100::globaltimer_ns() - t0 < 200000ull) {
+      ring.piece[0] = p.t.r0;
+      ring.piece[1] = (p.t.r1 - p.t.r0) * nh;
+      ring.piece[2] = p.q0;
+      ring.piece[3] = p.quanta - p.q1;
+    }
+    const int mine = p.units(warp), k0 = p.k0() + warp * kK8Keys, k1 = p.k1(), rows = (p.t.r1 - p.t.r0) * nh;
+    if (fresh) {
+      s_row = p.t.base + k0;
+      s_left = 2 * mine;
+      fresh = false;
+    }
+    left -= p.q1 - p.q0;
+    const int x1 = left > 0 && a.cut ? k8_next(a, n_x, x) : n_x;
+    const bool more = x1 < n_x;
+    send(kStages);
+    if (more) {                                        // the next piece, for the copies
+      const K8Piece n(a, x1, 0, left);
+      n_units = n.units(warp);
+      n_row = n.t.base + n.k0() + warp * kK8Keys;
+    }
+    float kn[2], vn[2];                                // scales of keys `lane` and lane + 32 of the next unit
+    auto load_scales = [&](int i) {
+      if (i < mine) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const size_t at = (size_t)((p.t.base + min(k0 + i * kK8Quantum + 32 * y + lane, k1 - 1)) >> a.c.shift) * a.c.G + g;
+          kn[y] = a.c.ks[at];
+          vn[y] = a.c.vs[at];
+        }
+      }
+    };
+    load_scales(0);
+    K8Rows r[NB];
+    float2 acc[NB][16];
+    uint32_t q_high[4][4];                             // high bytes of the first group, and of the second or nothing
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int m = min(b * 8 + gr, rows - 1);         // rows past the end repeat the last
+      k8_load_rows<T>(a, p.t.r0 + m / nh, h0 + m % nh, c, r[b]);
+#pragma unroll
+      for (int y = 0; y < 16; ++y) acc[b][y] = make_float2(0.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) q_high[i][y] = y & 1 ? (NB == 2 ? r[NB - 1].high[i][y >> 1] : k8_kept(0)) : r[0].high[i][y >> 1];
+    const int seen_by_all = min(p.t.len0, k1), seen_from = max(0, p.t.len1 - a.window);
+    for (int i = 0; i < mine; ++i) {
+      float s[NB][16];
+      const float km[2] = {kn[0], kn[1]}, vm[2] = {vn[0], vn[1]};
+      load_scales(i + 1);
+      const int key0 = k0 + i * kK8Quantum, ahead = i < mine - 1 ? kStages : kStages - 1;
+      failed = !sm100::mbar_wait_warp(&ring.full[warp][taken % kStages], (taken / kStages) & 1, gave_up);
+      if (failed) break;
+      k8_scores<NB>(stages + taken % kStages * kK8Stage, r, q_high, zero, s, gr, c);
+      sm100::fence_proxy_async_smem();                 // these reads before the copy that goes over them
+      __syncwarp();
+      ++taken;
+      send(ahead);
+      K8Weights w[NB];
+      float ks[16], vs[16];
+      k8_scales(km, a.c.shift, c, ks);
+      k8_scales(vm, a.c.shift, c, vs);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) k8_softmax(a, r[b], s[b], ks, vs, key0, c, key0 + kK8Keys > seen_by_all || key0 < seen_from, w[b]);
+      failed = !sm100::mbar_wait_warp(&ring.full[warp][taken % kStages], (taken / kStages) & 1, gave_up);
+      if (failed) break;
+      const uint32_t high[2][4] = {{w[0].high[0][0], NB == 2 ? w[NB - 1].high[0][0] : none[0], w[0].high[0][1], NB == 2 ? w[NB - 1].high[0][1] : none[1]},
+                                   {w[0].high[1][0], NB == 2 ? w[NB - 1].high[1][0] : none[2], w[0].high[1][1], NB == 2 ? w[NB - 1].high[1][1] : none[3]}};
+      k8_values<NB>(stages + taken % kStages * kK8Stage, w, high, zero, acc, gr, c);
+      sm100::fence_proxy_async_smem();
+      __syncwarp();
+      ++taken;
+      send(ahead);
+    }
+    if (failed) *gave_up = 1;
+    // the warps' shares, in the stage that no copy is on its way to
+    const int idle = (taken + kStages - 1) % kStages;
+    if (lane == 0) ring.free_stage[warp] = idle;
+    auto sums_of = [&](int w, int stage) { return reinterpret_cast<float*>(sm + (w * kStages + stage) * kK8Stage); };
+    auto stats_of = [&](int w, int stage) {
+      return K8Ring<NB>::kStatHere ? ring.stat + w * R : reinterpret_cast<float2*>(sm + (w * kStages + stage) * kK8Stage + K8Ring<NB>::kSumBytes);
+    };
+    float* sums = sums_of(warp, idle);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      r[b].l += __shfl_xor_sync(0xffffffffu, r[b].l, 1);
+      r[b].l += __shfl_xor_sync(0xffffffffu, r[b].l, 2);
+      const int m = b * 8 + gr;
+      if (c == 0) stats_of(warp, idle)[m] = make_float2(r[b].m, r[b].l);
+#pragma unroll
+      for (int y = 0; y < 16; y += 4) {
+        const int i = 8 * c + 2 * ((y >> 3) ^ (c & 1)) + (y >> 2 & 1);
+        *reinterpret_cast<float4*>(sums + k8_sum_at(m, i)) = make_float4(acc[b][y].x, acc[b][y + 1].x, acc[b][y + 2].x, acc[b][y + 3].x);
+        *reinterpret_cast<float4*>(sums + k8_sum_at(m, i + 4)) = make_float4(acc[b][y].y, acc[b][y + 1].y, acc[b][y + 2].y, acc[b][y + 3].y);
       }
     }
     __syncthreads();
-    return;
-  }
-  // the warps' shares: [warp][row] largest score | sum, then [warp][row][column]
-  constexpr int R = 8 * NB, LD = kK8Dim + 4;
-  float* stat = reinterpret_cast<float*>(sm);
-  float* sums = stat + 8 * R;
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const int m = warp * R + b * 8 + gr;
-    if (c == 0) {
-      stat[m] = r[b].m;
-      stat[4 * R + m] = r[b].l;
+    if (*gave_up) break;
+    const int r0 = ring.piece[0], n_rows = ring.piece[1], began = ring.piece[2], behind = ring.piece[3];
+    const bool whole = began == 0 && behind == 0;
+    float* slot = whole ? nullptr : a.part + ((size_t)blockIdx.x * 2 + (began == 0)) * R * LD;
+    if (!whole && began == 0 && threadIdx.x == 0) {    // its last quantum is the share's of which the first is not behind it
+      const long long last = (share + 1ll) * all / shares + behind - 1;
+      reinterpret_cast<K8Cut*>(a.part + (size_t)gridDim.x * 2 * R * LD)[blockIdx.x] = K8Cut{r0, n_rows, h0, nh, (int)(((last + 1) * shares - 1) / all) - share};
     }
+    const float* from[4];
+    const float2* stats[4];
 #pragma unroll
-    for (int x = 0; x < 16; x += 4) {
-      float* o = sums + m * LD + 32 * c + x;
-      *reinterpret_cast<float4*>(o) = make_float4(acc[b][x].x, acc[b][x + 1].x, acc[b][x + 2].x, acc[b][x + 3].x);
-      *reinterpret_cast<float4*>(o + 16) = make_float4(acc[b][x].y, acc[b][x + 1].y, acc[b][x + 2].y, acc[b][x + 3].y);
+    for (int y = 0; y < 4; ++y) {
+      const int stage = ring.free_stage[y];
+      from[y] = sums_of(y, stage);
+      stats[y] = stats_of(y, stage);
     }
-  }
-  __syncthreads();
-  for (int m = warp; m < t.rows; m += 4) {
-    float w[4], mx = -INFINITY, l = 0.f;
+    for (int m = warp; m < n_rows; m += 4) {
+      float w[4], mx = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) mx = fmaxf(mx, stat[x * R + m]);
-    const int h = t.head(m);
-    const size_t th = (size_t)t.token(m) * a.H + h;
-    const bool last = a.splits == 1;
-    const float sk = last && a.sink != nullptr ? a.sink[h] * kLog2e : -INFINITY, top = fmaxf(mx, sk), ref = top == -INFINITY ? 0.f : top;
+      for (int y = 0; y < 4; ++y) mx = fmaxf(mx, stats[y][m].x);
+      const int h = h0 + m % nh;
+      const float sk = whole && a.sink != nullptr ? a.sink[h] * kLog2e : -INFINITY, top = fmaxf(mx, sk), ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      w[x] = exp2f(stat[x * R + m] - ref);
-      l = fmaf(stat[(4 + x) * R + m], w[x], l);
-    }
-    float* part = nullptr;
-    float f = 1.f;
-    if (last) {
-      const float den = l + exp2f(sk - ref);
-      f = den == 0.f ? 0.f : 1.f / den;
-    } else {
-      part = a.part + (th * a.splits + blockIdx.z) * (a.c.dv + 2);
-      if (lane == 0) {
-        part[0] = mx;
-        part[1] = l;
+      for (int y = 0; y < 4; ++y) {
+        w[y] = exp2f(stats[y][m].x - ref);
+        l = fmaf(stats[y][m].y, w[y], l);
+      }
+      const float den = whole ? l + exp2f(sk - ref) : 1.f, f = den == 0.f ? 0.f : 1.f / den;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float4 v = *reinterpret_cast<const float4*>(from[y] + k8_sum_at(m, lane));
+        o = make_float4(fmaf(v.x, w[y], o.x), fmaf(v.y, w[y], o.y), fmaf(v.z, w[y], o.z), fmaf(v.w, w[y], o.w));
+      }
+      if (whole) {
+        k8_store_row<T>(a, r0 + m / nh, h, lane, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+      } else {
+        *reinterpret_cast<float4*>(slot + m * LD + 4 * lane) = o;
+        if (lane == 0) {
+          slot[m * LD + kK8Dim] = mx;
+          slot[m * LD + kK8Dim + 1] = l;
+        }
       }
     }
-    for (int x = lane; x < a.c.dv; x += 32) {
-      float o = 0.f;
-#pragma unroll
-      for (int y = 0; y < 4; ++y) o = fmaf(sums[(y * R + m) * LD + x], w[y], o);
-      if (last) reinterpret_cast<T*>(a.out)[th * a.c.dv + x] = from_f<T>(o * f);
-      else part[2 + x] = o;
+    if (!more) return;
+    sm100::fence_proxy_async_smem();                   // these reads before copies
+    __syncthreads();
+    x = x1;
+    q0 = 0;
+  }
+  // a copy did not arrive: those in flight land before the CTA ends
+  if (threadIdx.x == 0) {
+    atomicCAS(a.err, 0, kK8Wait);
+    const unsigned long long t0 = sm100::globaltimer_ns();
+    while (sm100::globaltimer_ns() - t0 < 200000ull) {
     }
   }
+  __syncthreads();
 }
 
-// A CTA a row and head: joins the ranges.  Those without a key have largest score -inf and sum 0.
-template <typename T>
-__global__ void __launch_bounds__(kK8Dim) attn_kv8_merge_kernel(const __grid_constant__ Kv8Attn a) {
+// Joins the pieces of the items that shares cut.  A CTA the item that begins in the share (and heads) of its number, if that one was cut.
+// A row has 32 / R warps, each with its share of the pieces: one long sequence has some fifty of them for a few rows, whose loads are to be under
+// way together (a warp a row took 22 us there).
+constexpr int kK8JoinThreads = 1024;
+template <typename T, int R>
+__global__ void __launch_bounds__(kK8JoinThreads) attn_kv8_join_kernel(const __grid_constant__ Kv8Attn a) {
   chain_enter();
-  __shared__ float weight[kK8MaxSplits];
-  const int t = blockIdx.x, h = blockIdx.y, step = a.c.dv + 2;
-  T* out = reinterpret_cast<T*>(a.out) + ((size_t)t * a.H + h) * a.c.dv;
-  if (a.cu != nullptr && t >= a.cu[a.n_seq]) {
-    if (threadIdx.x < a.c.dv) out[threadIdx.x] = from_f<T>(0.f);
-    return;
-  }
-  const float* pt = a.part + ((size_t)t * a.H + h) * a.splits * step;
-  if (threadIdx.x < 32) {
-    const int s0 = threadIdx.x, s1 = threadIdx.x + 32;
-    const float m0 = s0 < a.splits ? pt[(size_t)s0 * step] : -INFINITY, m1 = s1 < a.splits ? pt[(size_t)s1 * step] : -INFINITY;
-    const float l0 = s0 < a.splits ? pt[(size_t)s0 * step + 1] : 0.f, l1 = s1 < a.splits ? pt[(size_t)s1 * step + 1] : 0.f;
-    const float sk = a.sink != nullptr ? a.sink[h] * kLog2e : -INFINITY, top = fmaxf(warp_max(fmaxf(m0, m1)), sk), ref = top == -INFINITY ? 0.f : top;
-    const float e0 = exp2f(m0 - ref), e1 = exp2f(m1 - ref), den = warp_sum(l0 * e0 + l1 * e1) + exp2f(sk - ref), f = den == 0.f ? 0.f : 1.f / den;
-    weight[s0] = e0 * f;
-    weight[s1] = e1 * f;
+  constexpr int W = kK8JoinThreads / 32 / R;
+  __shared__ float4 sums[W][R][32];
+  __shared__ float stat[W][R];
+  const int hs = k8_groups(a.H, a.c.G);
+  const K8Cut cut = reinterpret_cast<const K8Cut*>(a.part + (size_t)gridDim.x * 2 * R * kK8SlotRow)[blockIdx.x];
+  const int m = (threadIdx.x >> 5) % R, part = (threadIdx.x >> 5) / R, lane = threadIdx.x & 31;
+  if (cut.more == 0) return;
+  const int pieces = cut.more + 1, h = cut.h0 + m % cut.nh;
+  auto slot = [&](int i) { return a.part + ((size_t)(blockIdx.x + i * hs) * 2 + (i == 0)) * R * kK8SlotRow + m * kK8SlotRow; };
+  if (m < cut.rows) {
+    float mx = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) mx = fmaxf(mx, slot(i)[kK8Dim]);
+    const float sk = a.sink != nullptr ? a.sink[h] * kLog2e : -INFINITY, top = fmaxf(warp_max(mx), sk), ref = top == -INFINITY ? 0.f : top;
+    float l = part == 0 && lane == 0 ? exp2f(sk - ref) : 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = part; i0 < pieces; i0 += W * 8) {
+      float4 v[8];
+      float w[8], x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float* s = slot(min(i0 + W * i, pieces - 1));
+        v[i] = *reinterpret_cast<const float4*>(s + 4 * lane);
+        w[i] = i0 + W * i < pieces ? s[kK8Dim] : -INFINITY;
+        x[i] = s[kK8Dim + 1];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool is = i0 + W * i < pieces;           // the last one again has no part
+        const float e = exp2f(w[i] - ref);
+        if (!is) continue;
+        o = make_float4(fmaf(v[i].x, e, o.x), fmaf(v[i].y, e, o.y), fmaf(v[i].z, e, o.z), fmaf(v[i].w, e, o.w));
+        if (lane == 0) l = fmaf(x[i], e, l);
+      }
+    }
+    sums[part][m][lane] = o;
+    if (lane == 0) stat[part][m] = l;
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < a.c.dv; x += kK8Dim) {
-    float o = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) o = fmaf(pt[(size_t)s * step + 2 + x], weight[s], o);
-    out[x] = from_f<T>(o);
+  if (m >= cut.rows || part != 0) return;
+  float4 o = sums[0][m][lane];
+  float den = stat[0][m];
+#pragma unroll
+  for (int y = 1; y < W; ++y) {
+    const float4 v = sums[y][m][lane];
+    o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+    den += stat[y][m];
   }
+  const float f = den == 0.f ? 0.f : 1.f / den;
+  k8_store_row<T>(a, cut.r0 + m / cut.nh, h, lane, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
 }
 
-// How a call runs: tokens of a tile, tiles of a sequence, ranges of keys.
+// How a call runs: tokens of a tile, tiles of a sequence, groups of 8 rows, CTAs, and whether their shares cut items.
 struct K8Plan {
-  int tt, tiles, splits, range, nb;
-  long long ctas;
+  int tt, tiles, nb, ctas, cut;
 };
-static K8Plan k8_plan(int n, int n_seq, int max_q, int H, int G, int d, int dv, int max_len, int window) {
+static K8Plan k8_plan(int n, int n_seq, int max_q, int H, int G, int max_len, int window) {
   K8Plan p{};
-  const int rep = H / G, groups = (rep + kK8Heads - 1) / kK8Heads, nh = std::min(rep, kK8Heads);
+  const int nh = std::min(H / G, kK8Heads);
   const bool one = n_seq <= 0 || max_q <= 1;
   p.tt = one ? 1 : std::max(1, std::min(max_q, 16 / nh));
   p.tiles = one ? 1 : (max_q + p.tt - 1) / p.tt;
   p.nb = p.tt * nh <= 8 ? 1 : 2;
-  p.ctas = (long long)(n_seq > 0 ? (long long)n_seq * p.tiles : n) * G * groups;
-  if (window > 0 && max_len > window + p.tt + kK8Keys) max_len = window + p.tt + kK8Keys;      // rows see windows that start apart, ranges at a unit
-  max_len = std::max(max_len, 1);
-  // Ranges: as many as two CTAs an SM have room for, of 4 units at least.
-  const long long most = std::min<long long>((max_len + 4 * kK8Keys - 1) / (4 * kK8Keys), kK8MaxSplits);
-  const long long s = std::max<long long>(1, std::min<long long>(most, 2 * kNumSMs / std::max<long long>(1, p.ctas)));
-  p.range = (int)(((max_len + s - 1) / s + kK8Keys - 1) / kK8Keys * kK8Keys);
-  p.splits = (max_len + p.range - 1) / p.range;
+  if (window > 0) max_len = std::min<long long>(max_len, (long long)window + p.tt + kK8Keys);      // rows see windows that start apart
+  const long long x = n_seq > 0 ? (long long)n_seq * p.tiles : n, hs = k8_groups(H, G), quanta = std::max(1, (max_len + kK8Quantum - 1) / kK8Quantum),
+                  resident = (long long)kNumSMs * (p.nb == 1 ? K8Ring<1>::kCtas : K8Ring<2>::kCtas);
+  p.cut = quanta > 1;
+  p.ctas = (int)std::min<long long>((p.cut ? std::min(std::max(1ll, resident / hs), x * quanta) : x) * hs, 0x7fffffff);
   return p;
 }
+static size_t k8_part_floats(const K8Plan& p) { return p.cut ? (size_t)p.ctas * (2 * 8 * p.nb * kK8SlotRow + sizeof(K8Cut) / 4) : 0; }
 
 int make_tmap_bytes_heads(CUtensorMap* map, const void* ptr, uint64_t dim, uint64_t heads, uint64_t rows, uint32_t box_rows);
 
@@ -647,13 +855,12 @@ template <typename T, int NB>
 static int launch_attn_kv8(const Kv8Attn& a, const K8Plan& p, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t stream) {
   static bool ready = false;
   if (!ready) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, kK8Smem);
+    const cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, k8_smem<NB>());
     if (e != cudaSuccess) return (int)e;
     ready = true;
   }
-  const int groups = (a.H / a.c.G + kK8Heads - 1) / kK8Heads;
-  launch_chained(attn_kv8_kernel<T, NB>, dim3(a.cu != nullptr ? a.n_seq * p.tiles : a.n, a.c.G * groups, p.splits), kK8Threads, kK8Smem, stream, tk, tv, a);
-  if (p.splits > 1) launch_chained(attn_kv8_merge_kernel<T>, dim3(a.n, a.H), kK8Dim, 0, stream, a);
+  launch_chained(attn_kv8_kernel<T, NB>, p.ctas, kK8Threads, k8_smem<NB>(), stream, tk, tv, a);
+  if (p.cut) launch_chained(attn_kv8_join_kernel<T, 8 * NB>, p.ctas, kK8JoinThreads, 0, stream, a);
   return launch_status();
 }
 
@@ -700,10 +907,9 @@ ELL_API int ell_kv8_read(const int8_t* kc, const int8_t* vc, const float* ks, co
 }
 
 // Scratch floats a call needs (0: none).  The sizes are those of ell_attn_kv8.
-ELL_API long long ell_attn_kv8_scratch(int n, int n_seq, int max_q, int H, int G, int d, int dv, int max_len, int window) {
+ELL_API long long ell_attn_kv8_scratch(int n, int n_seq, int max_q, int H, int G, int max_len, int window) {
   if (G <= 0 || H % G) return 0;
-  const K8Plan p = k8_plan(n, n_seq, max_q, H, G, d, dv, max_len, window);
-  return p.splits == 1 ? 0 : (long long)n * H * p.splits * (dv + 2);
+  return (long long)k8_part_floats(k8_plan(n, n_seq, max_q, H, G, max_len, window));
 }
 
 // q rows of ldq elements.  max_len bounds len[] (longer rows would be cut).  window: keys a row sees (<= 0: all).  cu [n_seq + 1] (or null): rows
@@ -712,14 +918,14 @@ ELL_API int ell_attn_kv8(const void* q, const int8_t* kc, const int8_t* vc, cons
                          const int* len, const float* sink, const float* slopes, const int* cu, int n, int n_seq, int max_q, int H, int G, int d, int dv,
                          int ldq, int max_len, int window, float scale, int shift, long long rows, int is_bf16, int* err, cudaStream_t stream) {
   if (n <= 0) return 0;
-  if (!k8_sizes_ok(G, d, dv, shift) || H % G || rows > 0x7fffffff || G * ((H / G + kK8Heads - 1) / kK8Heads) > 65535 || H > 65535) return -2;
+  if (!k8_sizes_ok(G, d, dv, shift) || H % G || rows > 0x7fffffff) return -2;
   if (cu == nullptr) n_seq = 0;
-  const K8Plan p = k8_plan(n, n_seq, max_q, H, G, d, dv, max_len, window);
-  if (p.splits > 1 && part == nullptr) return -2;
+  const K8Plan p = k8_plan(n, n_seq, max_q, H, G, max_len, window);
+  if (p.cut && (part == nullptr || !aligned_to(part, 16))) return -2;
   Kv8Attn a{};
   a.c = Kv8Cache{const_cast<int8_t*>(kc), const_cast<int8_t*>(vc), const_cast<float*>(ks), const_cast<float*>(vs), rows, G, d, dv, shift};
   a.q = q, a.out = out, a.part = part, a.base = base, a.len = len, a.cu = cu, a.sink = sink, a.slopes = slopes;
-  a.n = n, a.H = H, a.ldq = ldq, a.n_seq = n_seq, a.tiles = p.tiles, a.tt = p.tt, a.splits = p.splits, a.range = p.range;
+  a.n = n, a.H = H, a.ldq = ldq, a.n_seq = n_seq, a.tiles = p.tiles, a.tt = p.tt, a.cut = p.cut;
   a.window = window > 0 ? window : 0x3fffffff, a.scale = (float)((double)scale * 1.4426950408889634 / 2097152), a.err = err;
   CUtensorMap tk, tv;
   int rc = make_tmap_bytes_heads(&tk, kc, k8_row(d), G, rows, kK8Keys);

@@ -318,7 +318,7 @@ def attention_kv8(q, cache, base, length, max_len, scale, sink=None, alibi_slope
     with _on(q.device):
         out = torch.empty(T, H, cache.vdim, dtype=q.dtype, device=q.device)
         sl = cu._slopes(alibi_slopes, H, q.device)
-        need = lib().ell_attn_kv8_scratch(c_int(T), c_int(n_seq), c_int(max_q), c_int(H), *sizes, c_int(max_len), c_int(window or 0))
+        need = lib().ell_attn_kv8_scratch(c_int(T), c_int(n_seq), c_int(max_q), c_int(H), sizes[0], c_int(max_len), c_int(window or 0))
         part = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
         _check(lib().ell_attn_kv8(_p(q), *_kv8(cache), _p(out), _p(part), _p(base), _p(length), _p(None if sink is None else _f32(sink, "sink")), _p(sl),
                                   _p(cu_seqlens), c_int(T), c_int(n_seq), c_int(max_q), c_int(H), *sizes, c_int(_heads(q, "q")), c_int(max_len),
