@@ -34,102 +34,273 @@ __device__ __forceinline__ float k8_scale_of(float amax) {       // amax finite,
 }
 __device__ __forceinline__ float k8_nan() { return __int_as_float(0x7fffffff); }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // ---- writing -----------------------------------------------------------------------------------
-// A warp a block of a sequence, head, and keys or values.  Rows of the block that the step does not bring stay, requantised where the
-// scale grows.
+// A warp a block of a sequence, head, and keys or values, heads of a block next to each other.  L lanes a row, V elements each; up to kLoads
+// loads are under way together, and a block that fits them stays in registers between its maximum and its bytes.  Rows of the block that
+// the step does not bring stay, requantised where the scale grows.
+constexpr float kMagicF = 12582912.f;                             // 1.5 2^23: x + this has round(x) in its low bits
+// Low bytes of four words.
+__device__ __forceinline__ uint32_t k8_low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+template <bool TOP>
+__device__ __forceinline__ uint32_t k8_round(float x, float inv) {      // x inv is exact
+  return __float_as_uint(TOP ? fminf(fmaxf(x * inv, -127.f), 127.f) + kMagicF : fmaf(x, inv, kMagicF));
+}
+template <typename T, int V>
+struct K8Elems;
+template <>
+struct K8Elems<__nv_bfloat16, 8> {
+  static constexpr int kLoads = 8;
+  uint4 u;
+  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ float amax(float m) const {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max3_nan(m, __uint_as_float((w[i] & 0x7fffu) << 16), __uint_as_float(w[i] & 0x7fff0000u));
+    return m;
+  }
+  template <bool TOP>
+  __device__ __forceinline__ void store(int8_t* dst, float inv) const {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = k8_round<TOP>(__uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16), inv);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(k8_low_bytes(r[0], r[1], r[2], r[3]), k8_low_bytes(r[4], r[5], r[6], r[7]));
+  }
+};
+template <>
+struct K8Elems<float, 8> {
+  static constexpr int kLoads = 4;
+  float f[8];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 0.f;
+  }
+  __device__ __forceinline__ void load(const float* p) { load_v<8>(p, f); }
+  __device__ __forceinline__ float amax(float m) const {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) m = max3_nan(m, fabsf(f[i]), fabsf(f[i + 1]));
+    return m;
+  }
+  template <bool TOP>
+  __device__ __forceinline__ void store(int8_t* dst, float inv) const {
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = k8_round<TOP>(f[i], inv);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(k8_low_bytes(r[0], r[1], r[2], r[3]), k8_low_bytes(r[4], r[5], r[6], r[7]));
+  }
+};
 template <typename T>
-__global__ void __launch_bounds__(256) kv8_append_kernel(const Kv8Cache c, const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ base_,
-                                                         const int* __restrict__ len_, const int* __restrict__ cu, int n_seq, int n, int blocks,
-                                                         int ldk, int ldv, int* __restrict__ err) {
+struct K8Elems<T, 1> {
+  static constexpr int kLoads = 8;
+  float f;
+  __device__ __forceinline__ void zero() { f = 0.f; }
+  __device__ __forceinline__ void load(const T* p) { f = to_f<T>(*p); }
+  __device__ __forceinline__ float amax(float m) const { return max_nan(m, fabsf(f)); }
+  template <bool TOP>
+  __device__ __forceinline__ void store(int8_t* dst, float inv) const { *dst = (int8_t)k8_round<TOP>(f, inv); }
+};
+
+template <typename T, int V>
+__global__ void __launch_bounds__(256, 4) kv8_append_kernel(const Kv8Cache c, const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ base_,
+                                                            const int* __restrict__ len_, const int* __restrict__ cu, int n_seq, int n, int blocks,
+                                                            int ldk, int ldv, int* __restrict__ err) {
   chain_enter(k, v, base_, len_, cu, err);
-  const long long item = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, g = (int)(item % c.G);
-  const long long rest = item / c.G;
-  const int which = (int)(rest & 1), j = (int)((rest >> 1) % blocks);
-  const long long s = (rest >> 1) / blocks;
+  const unsigned item = blockIdx.x * 8u + (threadIdx.x >> 5), rest = item / c.G;
+  const int lane = threadIdx.x & 31, g = (int)(item % c.G), which = (int)(rest & 1), j = (int)((rest >> 1) % blocks), s = (int)((rest >> 1) / blocks);
   if (s >= n_seq) return;
   const int r0 = cu[s], count = min(cu[s + 1], n) - r0;
   if (count <= 0 || r0 < 0) return;
   const int base = base_[r0], p0 = len_[r0] - 1;
-  if (p0 < 0) return;                                             // a padding row
-  const int b = (p0 >> c.shift) + j, first = max(p0, b << c.shift), last = min(p0 + count, (b + 1) << c.shift);
+  if (p0 < 0) return;                                             // padding
+  const int b = (p0 >> c.shift) + j, start = b << c.shift, first = max(p0, start), last = min(p0 + count, start + (1 << c.shift));
   if (first >= last) return;
   if (!k8_inside(c, base, p0 + count)) {
     if (lane == 0) atomicCAS(err, 0, kK8Place);
     return;
   }
-  const int width = which ? c.dv : c.d, row = k8_row(width), ld = which ? ldv : ldk;
-  const T* src = (which ? v : k) + (size_t)r0 * ld + (size_t)g * width;
-  int8_t* dst = (which ? c.v : c.k) + ((size_t)base * c.G + g) * row;
+  const int width = which ? c.dv : c.d, row = k8_row(width), step = c.G * row, rows = last - first;
+  const size_t ld = which ? ldv : ldk;
+  const T* src = (which ? v : k) + (size_t)(r0 + first - p0) * ld + (size_t)g * width;
   float* scale = (which ? c.vs : c.ks) + ((size_t)(base >> c.shift) + b) * c.G + g;
-  float amax = 0.f;
-  bool odd = false;
-  for (int p = first; p < last; ++p)
-    for (int x = lane; x < width; x += 32) {
-      const float f = fabsf(to_f<T>(src[(size_t)(p - p0) * ld + x]));
-      odd = odd || !(f <= 3.4028235e38f);
-      amax = fmaxf(amax, f);
+  const float old = first > start ? *scale : 0.f;
+  int8_t* dst = (which ? c.v : c.k) + ((size_t)base * c.G + g) * row;
+  int shift = 0;                                                  // lanes of a row: a power of two
+  while ((V << shift) < row && shift < 5) ++shift;
+  const int per = 32 >> shift, my_row = lane >> shift, piece = lane & ((1 << shift) - 1);
+  constexpr int kLoads = K8Elems<T, V>::kLoads;
+  const int turns = V == 1 ? (row + 31) / 32 : 1, chunk = per * kLoads;      // single elements of a row take several turns
+  const bool kept = rows <= chunk && turns == 1;
+  K8Elems<T, V> e[kLoads];
+  auto load = [&](int at, int r) {
+    const T* from = src + (size_t)(r + my_row) * ld + at;
+    const int mine = at < width ? rows - r - my_row : 0;          // rows of this lane, one of `per`
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      e[i].zero();
+      if (i * per < mine) e[i].load(from + (size_t)(i * per) * ld);
     }
-  odd = __any_sync(0xffffffffu, odd);
-  float now = odd ? k8_nan() : k8_scale_of(warp_max(amax));
-  const int start = b << c.shift;
+  };
+  float amax = 0.f;
+  for (int x = 0; x < turns; ++x)
+    for (int r = 0; r < rows; r += chunk) {
+      load(x * 32 + piece * V, r);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) amax = e[i].amax(amax);
+    }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  float now = amax <= 3.4028235e38f ? k8_scale_of(amax) : k8_nan();
   if (first > start) {                                            // rows that were there
-    const float old = *scale;
     const bool grows = !(old >= now);
-    if (old != old || odd) now = k8_nan();
+    if (old != old) now = old;
     else if (!grows) now = old;
     if (grows && now == now) {
-      const float f = old / now;
+      const float ratio = old / now;
       for (int p = start; p < first; ++p)
-        for (int x = lane; x < row; x += 32) {
-          int8_t* q = dst + (size_t)p * c.G * row + x;
-          *q = (int8_t)__float2int_rn((float)*q * f);
+        for (int x = lane * 4; x < row; x += 128) {
+          uint32_t* q = reinterpret_cast<uint32_t*>(dst + (size_t)p * step + x);
+          const uint32_t w = *q;
+          uint32_t z[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) z[i] = k8_round<false>((float)(int8_t)(w >> (8 * i)), ratio);
+          *q = k8_low_bytes(z[0], z[1], z[2], z[3]);
         }
     }
   }
-  const float inv = 1.f / now;                                    // a power of two
-  for (int p = first; p < last; ++p)
-    for (int x = lane; x < row; x += 32) {
-      float f = 0.f;
-      if (x < width && now == now) f = fminf(fmaxf(to_f<T>(src[(size_t)(p - p0) * ld + x]) * inv, -127.f), 127.f);
-      dst[(size_t)p * c.G * row + x] = (int8_t)__float2int_rn(f);
+  const bool none = now != now, top = now == k8_scale_of(3.4028235e38f);
+  const float inv = none ? 0.f : 1.f / now;                       // a power of two
+  for (int x = 0; x < turns; ++x)
+    for (int r = 0; r < rows; r += chunk) {
+      const int at = x * 32 + piece * V;
+      if (!kept) load(at, r);
+      if (none) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) e[i].zero();
+      }
+      int8_t* to = dst + (size_t)(first + r + my_row) * step + at;
+      const int mine = at < row ? rows - r - my_row : 0;          // rows of this lane, one of `per`
+      if (top) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          if (i * per < mine) e[i].template store<true>(to + (size_t)(i * per) * step, inv);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          if (i * per < mine) e[i].template store<false>(to + (size_t)(i * per) * step, inv);
+      }
     }
   __syncwarp();                                                   // everybody has read the old scale
   if (lane == 0) *scale = now;
 }
 
 // ---- reading back ------------------------------------------------------------------------------
-// ko [n, max_len, G, d], vo [n, max_len, G, dv]: rows base[i] .. base[i] + len[i] - 1, then zeros.  Eight values a thread (V) or one.
+// Bytes times a scale: a byte and 128 is put into the mantissa of 2^23, from which 2^23 + 128 is taken (an integer's own conversion has a
+// quarter of this rate).  The products are exact in bf16 too: their upper halves.
+template <int V, typename T>
+__device__ __forceinline__ void k8_store_values(T* o, const uint32_t* w, float s) {
+  constexpr bool kHalf = sizeof(T) == 2;
+  if (V == 8) {
+    float2 f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = w[i / 2] ^ 0x80808080u;
+      f[i] = make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, i & 1 ? 0x7552 : 0x7550)), __uint_as_float(__byte_perm(u, 0x4b000000u, i & 1 ? 0x7553 : 0x7551)));
+      f[i] = sm100::fmul2(sm100::fadd2(f[i], make_float2(-8388736.f, -8388736.f)), make_float2(s, s));
+    }
+    if (kHalf) {
+      uint4 z;
+      z.x = __byte_perm(__float_as_uint(f[0].x), __float_as_uint(f[0].y), 0x7632);
+      z.y = __byte_perm(__float_as_uint(f[1].x), __float_as_uint(f[1].y), 0x7632);
+      z.z = __byte_perm(__float_as_uint(f[2].x), __float_as_uint(f[2].y), 0x7632);
+      z.w = __byte_perm(__float_as_uint(f[3].x), __float_as_uint(f[3].y), 0x7632);
+      *reinterpret_cast<uint4*>(o) = z;
+    } else {
+      reinterpret_cast<float4*>(o)[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+      reinterpret_cast<float4*>(o)[1] = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
+    }
+  } else {
+    *o = from_f<T>((float)(int8_t)w[0] * s);
+  }
+}
+// ko [n, max_len, G, d], vo [n, max_len, G, dv].  cu null: rows base[i] .. base[i] + len[i] - 1 of the cache, then zeros.  Otherwise sequence i has
+// the query rows cu[i] .. cu[i + 1] - 1 with base and len of their own: its rows are those that its last one sees, nothing is written behind them,
+// and row_base[r] becomes the place of a query row's keys in ko.  A thread keeps its place in a row, V elements, and takes `chunk` positions.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Cache c, T* __restrict__ ko, T* __restrict__ vo, const int* __restrict__ base,
-                                                       const int* __restrict__ len, int max_len, int* __restrict__ err) {
-  chain_enter(ko, vo, base, len, err);
-  const int i = blockIdx.y, first = base[i], n = min(len[i], max_len), pk = c.d / V, pv = c.dv / V, per = c.G * (pk + pv);
+                                                       const int* __restrict__ len, const int* __restrict__ cu, int* __restrict__ row_base, int rows, int max_len,
+                                                       int chunk, int* __restrict__ err) {
+  chain_enter(ko, vo, base, len, cu, row_base, err);
+  const int i = blockIdx.y, pk = c.d / V, pv = c.dv / V, per = c.G * (pk + pv);
+  int r0 = i, r1 = i + 1;
+  if (cu != nullptr) {
+    r0 = cu[i];
+    r1 = min(cu[i + 1], rows);
+    if (r0 >= r1) return;
+    if (blockIdx.x == 0)
+      for (int r = r0 + threadIdx.x; r < r1; r += 256) row_base[r] = i * max_len;
+  }
+  const int first = base[r0], n = min(len[r1 - 1], max_len);
   const bool ok = n <= 0 || k8_inside(c, first, n);
   if (!ok && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(err, 0, kK8Place);
-  for (long long x = blockIdx.x * 256ll + threadIdx.x; x < (long long)max_len * per; x += gridDim.x * 256ll) {
-    const int p = (int)(x / per), y = (int)(x % per);
-    const bool is_v = y >= c.G * pk;
-    const int z = is_v ? y - c.G * pk : y, pieces = is_v ? pv : pk, width = is_v ? c.dv : c.d, g = z / pieces, at = z % pieces * V;
-    float f[V];
+  const int p0 = blockIdx.x * chunk, p1 = min(p0 + chunk, cu != nullptr && ok ? n : max_len);
+  const int beside = max(1, 256 / per);                          // positions that the threads take side by side
+  for (int y = threadIdx.x; y < beside * per; y += 256) {
+    const int z0 = y % per, at_p = y / per;
+    const bool is_v = z0 >= c.G * pk;
+    const int z = is_v ? z0 - c.G * pk : z0, pieces = is_v ? pv : pk, width = is_v ? c.dv : c.d, g = z / pieces, at = z % pieces * V, row = k8_row(width);
+    const int step = c.G * row, out_step = c.G * width, mine = ok ? min(n, p1) : 0;
+    const int8_t* q = (is_v ? c.v : c.k) + ((size_t)first * c.G + g) * row + at;
+    const float* scale = (is_v ? c.vs : c.ks) + (size_t)(first >> c.shift) * c.G + g;
+    T* o = (is_v ? vo : ko) + ((size_t)i * max_len * c.G + g) * width + at;
+    constexpr int kLoads = V == 8 ? 8 : 4;
+    int p = p0 + at_p;
+    for (; p < mine; p += kLoads * beside) {
+      uint32_t w[kLoads][V == 8 ? 2 : 1];
+      float s[kLoads];
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = 0.f;
-    if (ok && p < n) {
-      const size_t row = (size_t)first + p;
-      const int8_t* q = (is_v ? c.v : c.k) + (row * c.G + g) * k8_row(width) + at;
-      const float s = (is_v ? c.vs : c.ks)[(row >> c.shift) * c.G + g];
-      if (V == 8) {
-        const uint2 u = *reinterpret_cast<const uint2*>(q);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)((e < 4 ? u.x : u.y) >> (8 * (e & 3))) * s;
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = (float)q[e] * s;
+      for (int x = 0; x < kLoads; ++x) {
+        const int r = min(p + x * beside, mine - 1);
+        s[x] = scale[(size_t)(r >> c.shift) * c.G];
+        if (V == 8) {
+          const uint2 u = *reinterpret_cast<const uint2*>(q + (size_t)r * step);
+          w[x][0] = u.x;
+          w[x][V == 8] = u.y;
+        } else {
+          w[x][0] = (uint8_t)q[(size_t)r * step];
+        }
       }
+#pragma unroll
+      for (int x = 0; x < kLoads; ++x)
+        if (p + x * beside < mine) k8_store_values<V>(o + (size_t)(p + x * beside) * out_step, w[x], s[x]);
     }
-    T* o = (is_v ? vo : ko) + (((size_t)i * max_len + p) * c.G + g) * width + at;
-    store_v<V>(o, f);
+    for (p = max(p0, (mine - p0 - at_p + beside - 1) / beside * beside + p0) + at_p; p < p1; p += beside) {      // behind the sequence
+      const float none[V] = {};
+      store_v<V>(o + (size_t)p * out_step, none);
+    }
   }
+}
+
+// Rows that see nothing, and those behind the last sequence, of out [n, width]: zero.
+__global__ void __launch_bounds__(256) kv8_clear_kernel(__nv_bfloat16* __restrict__ out, const int* __restrict__ len, const int* __restrict__ cu, int n_seq, int n, int width) {
+  chain_enter(out, len, cu);
+  const int end = cu[n_seq];
+  for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < n; t += gridDim.x * 8)
+    if (t >= end || len[t] <= 0)
+      for (int x = threadIdx.x & 31; x < width; x += 32) out[(size_t)t * width + x] = __float2bfloat16_rn(0.f);
 }
 
 // ---- attention -----------------------------------------------------------------------------------
@@ -247,7 +418,6 @@ __device__ __forceinline__ void k8_store_row(const Kv8Attn& a, int tok, int h, i
 
 // The sums start at 12582912 = 1.5 2^23 taken as bits: a sum below 2^22 read as a float is then 12582912 + sum, and a subtraction converts it.
 constexpr uint32_t kMagic = 0x4b400000;
-constexpr float kMagicF = 12582912.f;
 // The left operand signed (queries) or not (weights).  `first`: a sum that starts here, from `zero`.
 template <bool SIGNED>
 __device__ __forceinline__ void mma_i8(int (&c)[4], bool first, const uint32_t (&zero)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -279,16 +449,6 @@ __device__ __forceinline__ float2 k8_sum(int x, int y) { return sm100::fadd2(mak
 __device__ __forceinline__ float2 k8_join(int l0, int l1, int m0, int m1, int h0, int h1) {
   const float2 b = make_float2(256.f, 256.f);
   return sm100::ffma2(sm100::ffma2(k8_sum(h0, h1), b, k8_sum(m0, m1)), b, k8_sum(l0, l1));
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
 }
 // Bytes of 4 x 4: x[i] byte j -> x[j] byte i.
 __device__ __forceinline__ void transpose_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&y)[4]) {
@@ -880,29 +1040,42 @@ ELL_API int ell_kv8_append(int8_t* kc, int8_t* vc, float* ks, float* vs, const v
   if (n <= 0 || n_seq <= 0 || max_new <= 0) return 0;
   if (!k8_sizes_ok(G, d, dv, shift)) return -2;
   const Kv8Cache c{kc, vc, ks, vs, rows, G, d, dv, shift};
-  const int block = 1 << shift;
+  const int block = 1 << shift, esz = is_bf16 ? 2 : 4;
   const long long blocks = ((long long)max_new + 2 * block - 2) / block, ctas = ((long long)n_seq * blocks * 2 * G + 7) / 8;
-  if (ctas > 0x7fffffff) return -2;
-  if (is_bf16)
-    launch_chained(kv8_append_kernel<__nv_bfloat16>, (unsigned)ctas, 256, 0, stream, c, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, base, len, cu,
-                   n_seq, n, (int)blocks, ldk, ldv, err);
-  else
-    launch_chained(kv8_append_kernel<float>, (unsigned)ctas, 256, 0, stream, c, (const float*)k, (const float*)v, base, len, cu, n_seq, n, (int)blocks,
-                   ldk, ldv, err);
+  if (ctas > 0x0fffffff) return -2;
+  const bool vec = d % 8 == 0 && dv % 8 == 0 && ldk * esz % 16 == 0 && ldv * esz % 16 == 0 && aligned_to(k, 16) && aligned_to(v, 16);
+#define ELL_APPEND(T, V)                                                                                                                                   \
+  launch_chained(kv8_append_kernel<T, V>, (unsigned)ctas, 256, 0, stream, c, (const T*)k, (const T*)v, base, len, cu, n_seq, n, (int)blocks, ldk, ldv, err)
+  if (is_bf16) vec ? ELL_APPEND(__nv_bfloat16, 8) : ELL_APPEND(__nv_bfloat16, 1);
+  else vec ? ELL_APPEND(float, 8) : ELL_APPEND(float, 1);
+#undef ELL_APPEND
   return launch_status();
 }
 
+// cu [n + 1] and row_base [rows_q] (or null, null): see kv8_read_kernel.
 ELL_API int ell_kv8_read(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, void* ko, void* vo, const int* base, const int* len,
-                         int n, int max_len, int G, int d, int dv, int shift, long long rows, int is_bf16, int* err, cudaStream_t stream) {
+                         const int* cu, int* row_base, int n, int rows_q, int max_len, int G, int d, int dv, int shift, long long rows, int is_bf16, int* err,
+                         cudaStream_t stream) {
   if (n <= 0 || max_len <= 0) return 0;
-  if (!k8_sizes_ok(G, d, dv, shift) || n > 65535) return -2;
+  if (!k8_sizes_ok(G, d, dv, shift) || n > 65535 || (cu != nullptr && (long long)n * max_len > 0x7fffffff)) return -2;
   const Kv8Cache c{const_cast<int8_t*>(kc), const_cast<int8_t*>(vc), const_cast<float*>(ks), const_cast<float*>(vs), rows, G, d, dv, shift};
-  const bool vec = d % 8 == 0 && dv % 8 == 0;
-  const dim3 grid(grid_for((long long)max_len * G * (d + dv) / (vec ? 8 : 1), 256, std::max(1, 16 / n)), n);
-#define ELL_READ(T, V) launch_chained(kv8_read_kernel<T, V>, grid, 256, 0, stream, c, (T*)ko, (T*)vo, base, len, max_len, err)
-  if (is_bf16) vec ? ELL_READ(__nv_bfloat16, 8) : ELL_READ(__nv_bfloat16, 1);
-  else vec ? ELL_READ(float, 8) : ELL_READ(float, 1);
+  const int vec = d % 8 == 0 && dv % 8 == 0 ? 8 : 1;
+  // positions of a CTA: sixteen turns of its threads, fewer where that leaves SMs without work
+  const int per = G * (d + dv) / vec, beside = std::max(1, 256 / per);
+  const long long most = (long long)n * max_len / (8 * kNumSMs) + 1;
+  const int chunk = (int)std::max<long long>(beside, std::min<long long>(16 * beside, most / beside * beside));
+  const dim3 grid((max_len + chunk - 1) / chunk, n);
+#define ELL_READ(T, V) launch_chained(kv8_read_kernel<T, V>, grid, 256, 0, stream, c, (T*)ko, (T*)vo, base, len, cu, row_base, rows_q, max_len, chunk, err)
+  if (is_bf16) vec == 8 ? ELL_READ(__nv_bfloat16, 8) : ELL_READ(__nv_bfloat16, 1);
+  else vec == 8 ? ELL_READ(float, 8) : ELL_READ(float, 1);
 #undef ELL_READ
+  return launch_status();
+}
+
+// out bf16 [n, width]
+ELL_API int ell_kv8_clear(void* out, const int* len, const int* cu, int n_seq, int n, int width, cudaStream_t stream) {
+  if (n <= 0) return 0;
+  launch_chained(kv8_clear_kernel, grid_for((long long)n * 32, 256, 4), 256, 0, stream, (__nv_bfloat16*)out, len, cu, n_seq, n, width);
   return launch_status();
 }
 

@@ -306,15 +306,37 @@ def kv8_read(cache, base, length, max_len, dtype):
     sizes, place = _kv8_sizes(cache)
     with _on(dev):
         out = [torch.empty(n, max_len, cache.k.shape[1], w, dtype=dtype, device=dev) for w in (cache.dim, cache.vdim)]
-        _check(lib().ell_kv8_read(*_kv8(cache), _p(out[0]), _p(out[1]), _p(base), _p(length), c_int(n), c_int(max_len), *sizes, *place, _bf(dtype),
+        _check(lib().ell_kv8_read(*_kv8(cache), _p(out[0]), _p(out[1]), _p(base), _p(length), _p(None), _p(None), c_int(n), c_int(n), c_int(max_len), *sizes, *place, _bf(dtype),
                                   _p(err_flag(dev)), _stream()), "kv8_read")
     return out[0], out[1]
 
 
+# Continued prompts: with this many rows (tokens times query heads of a key head) of a sequence, the cache's rows are written out in bf16 once
+# and the tcgen05 kernel attends to those; that takes memory for them.
+KV8_READ_ROWS, KV8_READ_BYTES = 512, 1 << 30
+
+
+def _attention_read_back(q, cache, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):
+    T, G, n, dev = q.shape[0], cache.k.shape[1], cu_seqlens.numel() - 1, q.device
+    sizes, place = _kv8_sizes(cache)
+    k, v = (torch.empty(n * max_len, G, w, dtype=q.dtype, device=dev) for w in (cache.dim, cache.vdim))
+    rows = torch.empty(T, dtype=torch.int32, device=dev)
+    _check(lib().ell_kv8_read(*_kv8(cache), _p(k), _p(v), _p(base), _p(length), _p(cu_seqlens), _p(rows), c_int(n), c_int(T), c_int(max_len), *sizes, *place,
+                              _bf(q.dtype), _p(err_flag(dev)), _stream()), "kv8_read")
+    out = attention_rows(q, k, v, rows, length, max_len, scale, sink, alibi_slopes, window, None, cu_seqlens, max_q)
+    _check(lib().ell_kv8_clear(_p(out), _p(length), _p(cu_seqlens), c_int(n), c_int(T), c_int(out[0].numel()), _stream()), "kv8_clear")
+    return out
+
+
 def attention_kv8(q, cache, base, length, max_len, scale, sink=None, alibi_slopes=None, window=None, cu_seqlens=None, max_q=None):
-    T, H, _ = q.shape
+    T, H, d = q.shape
     n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, max_q)
     sizes, place = _kv8_sizes(cache)
+    G = cache.k.shape[1]
+    if max_q * (H // G) >= KV8_READ_ROWS and q.dtype == torch.bfloat16 and not ((d | cache.vdim) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4) and \
+            2 * n_seq * max_len * G * (d + cache.vdim) <= KV8_READ_BYTES:
+        with _on(q.device):
+            return _attention_read_back(q, cache, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
     with _on(q.device):
         out = torch.empty(T, H, cache.vdim, dtype=q.dtype, device=q.device)
         sl = cu._slopes(alibi_slopes, H, q.device)
