@@ -1079,22 +1079,17 @@ ELL_API int ell_kv8_clear(void* out, const int* len, const int* cu, int n_seq, i
   return launch_status();
 }
 
-// Scratch floats a call needs (0: none).  The sizes are those of ell_attn_kv8.
-ELL_API long long ell_attn_kv8_scratch(int n, int n_seq, int max_q, int H, int G, int max_len, int window) {
-  if (G <= 0 || H % G) return 0;
-  return (long long)k8_part_floats(k8_plan(n, n_seq, max_q, H, G, max_len, window));
-}
-
-// q rows of ldq elements.  max_len bounds len[] (longer rows would be cut).  window: keys a row sees (<= 0: all).  cu [n_seq + 1] (or null): rows
+// q rows of ldq elements.  max_len bounds len[].  part (16-byte aligned): `part_floats` of scratch where max_len is above 256, enough for
+// max(444, key heads x groups of 16 query heads) x 4232.  window: keys a row sees (<= 0: all).  cu [n_seq + 1] (or null): rows
 // cu[i] .. cu[i + 1] - 1 are consecutive tokens of one sequence, with one base and lengths that grow by one; max_q bounds their number.
-ELL_API int ell_attn_kv8(const void* q, const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, void* out, float* part, const int* base,
-                         const int* len, const float* sink, const float* slopes, const int* cu, int n, int n_seq, int max_q, int H, int G, int d, int dv,
+ELL_API int ell_attn_kv8(const void* q, const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, void* out, float* part, long long part_floats,
+                         const int* base, const int* len, const float* sink, const float* slopes, const int* cu, int n, int n_seq, int max_q, int H, int G, int d, int dv,
                          int ldq, int max_len, int window, float scale, int shift, long long rows, int is_bf16, int* err, cudaStream_t stream) {
   if (n <= 0) return 0;
   if (!k8_sizes_ok(G, d, dv, shift) || H % G || rows > 0x7fffffff) return -2;
   if (cu == nullptr) n_seq = 0;
   const K8Plan p = k8_plan(n, n_seq, max_q, H, G, max_len, window);
-  if (p.cut && (part == nullptr || !aligned_to(part, 16))) return -2;
+  if (p.cut && (part == nullptr || !aligned_to(part, 16) || (size_t)part_floats < k8_part_floats(p))) return -2;
   Kv8Attn a{};
   a.c = Kv8Cache{const_cast<int8_t*>(kc), const_cast<int8_t*>(vc), const_cast<float*>(ks), const_cast<float*>(vs), rows, G, d, dv, shift};
   a.q = q, a.out = out, a.part = part, a.base = base, a.len = len, a.cu = cu, a.sink = sink, a.slopes = slopes;

@@ -2,8 +2,8 @@
 and the tcgen05 GEMM / attention) for bf16 and fp32 CUDA tensors; the signatures are those of ``ops.infer``."""
 from __future__ import annotations
 
-from contextlib import nullcontext
-from ctypes import addressof, c_float, c_int, c_longlong
+import functools
+from ctypes import addressof, c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -280,71 +280,115 @@ def attention_rows(q, k, v, base, length, max_len, scale, sink=None, alibi_slope
 
 
 # ---- a cache held in 8 bits ------------------------------------------------------------------------
-def _kv8(cache):
-    return [_p(t) for t in cache[:4]]
+# A decoding step calls these for every layer, and a short context's kernels take less time than a call from Python: the arguments go over
+# as numbers (a ctypes object each costs 0.2 us), types are declared once.
+_KV8_TYPES = {
+    "ell_kv8_append": "pppp pp ppp iii iii ii il i pp", "ell_kv8_read": "pppp pp pp pp iii iii il i pp", "ell_kv8_clear": "p pp iii p",
+    "ell_attn_kv8": "p pppp pp l pp pp p iii i iii i ii f il i pp"}
+_KV8_FNS, _ERR_WORDS = {}, {}
 
 
-def _kv8_sizes(cache):
-    return [c_int(cache.k.shape[1]), c_int(cache.dim), c_int(cache.vdim)], [c_int(cache.block.bit_length() - 1), c_longlong(cache.k.shape[0])]
+def _kv8_fn(name):
+    f = _KV8_FNS.get(name)
+    if f is None:
+        f = getattr(lib(), name)
+        f.argtypes = [{"p": c_void_p, "i": c_int, "l": c_longlong, "f": c_float}[t] for t in _KV8_TYPES[name].replace(" ", "")]
+        _KV8_FNS[name] = f
+    return f
 
 
-def _on(device):
-    """The context in which ``device`` is the current one."""
-    return nullcontext() if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+def _err_word(device):
+    p = _ERR_WORDS.get(device.index)
+    if p is None:
+        p = _ERR_WORDS[device.index] = err_flag(device).data_ptr()
+    return p
 
 
-def kv8_append(cache, k, v, base, length, cu_seqlens, max_new):
-    sizes, place = _kv8_sizes(cache)
-    with _on(k.device):
-        _check(lib().ell_kv8_append(*_kv8(cache), _p(k), _p(v), _p(base), _p(length), _p(cu_seqlens), c_int(k.shape[0]),
-                                    c_int(cu_seqlens.numel() - 1), c_int(max_new), *sizes, c_int(_heads(k, "k")), c_int(_heads(v, "v")), *place,
-                                    _bf(k.dtype), _p(err_flag(k.device)), _stream()), "kv8_append")
+def _on_device(f):
+    """``f(tensor, ...)`` with the tensor's device as the current one."""
+    @functools.wraps(f)
+    def call(t, *args):
+        if t.get_device() == torch._C._cuda_getDevice():
+            return f(t, *args)
+        with torch.cuda.device(t.device):
+            return f(t, *args)
+    return call
 
 
-def kv8_read(cache, base, length, max_len, dtype):
-    n, dev = base.numel(), cache.k.device
-    sizes, place = _kv8_sizes(cache)
-    with _on(dev):
-        out = [torch.empty(n, max_len, cache.k.shape[1], w, dtype=dtype, device=dev) for w in (cache.dim, cache.vdim)]
-        _check(lib().ell_kv8_read(*_kv8(cache), _p(out[0]), _p(out[1]), _p(base), _p(length), _p(None), _p(None), c_int(n), c_int(n), c_int(max_len), *sizes, *place, _bf(dtype),
-                                  _p(err_flag(dev)), _stream()), "kv8_read")
-    return out[0], out[1]
+def _kv8_parts(cache):
+    """Arguments: addresses | heads, sizes | rows of a block as a shift, rows."""
+    k, v, ks, vs, d, dv = cache
+    R, G = k.shape[0], k.shape[1]
+    return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()), (G, d, dv), ((R // ks.shape[0]).bit_length() - 1, R)
+
+
+def _packed(t, name):
+    """``_heads``, in fewer steps."""
+    (T, H, d), (ld, heads, one) = t.shape, t.stride()
+    if one == 1 and (heads == d or H == 1) and T > 1:
+        return ld
+    return _heads(t, name)
+
+
+def _is_bf(dtype):
+    return 1 if dtype is torch.bfloat16 else 0
+
+
+@_on_device
+def kv8_append(k, v, cache, base, length, cu_seqlens, max_new):
+    data, sizes, place = _kv8_parts(cache)
+    _check(_kv8_fn("ell_kv8_append")(*data, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(), k.shape[0],
+                                     cu_seqlens.numel() - 1, max_new, *sizes, _packed(k, "k"), _packed(v, "v"), *place, _is_bf(k.dtype),
+                                     _err_word(k.device), _stream()), "kv8_append")
+
+
+@_on_device
+def kv8_read(base, length, cache, max_len, dtype):
+    n, (data, sizes, place) = base.numel(), _kv8_parts(cache)
+    G, d, dv = sizes
+    k = torch.empty((n, max_len, G, d), dtype=dtype, device=base.device)
+    v = torch.empty_like(k) if d == dv else k.new_empty((n, max_len, G, dv))
+    _check(_kv8_fn("ell_kv8_read")(*data, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), None, None, n, n, max_len, *sizes, *place,
+                                   _is_bf(dtype), _err_word(base.device), _stream()), "kv8_read")
+    return k, v
 
 
 # Continued prompts: with this many rows (tokens times query heads of a key head) of a sequence, the cache's rows are written out in bf16 once
 # and the tcgen05 kernel attends to those; that takes memory for them.
 KV8_READ_ROWS, KV8_READ_BYTES = 512, 1 << 30
+KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 256, 444, 4232
 
 
 def _attention_read_back(q, cache, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):
-    T, G, n, dev = q.shape[0], cache.k.shape[1], cu_seqlens.numel() - 1, q.device
-    sizes, place = _kv8_sizes(cache)
-    k, v = (torch.empty(n * max_len, G, w, dtype=q.dtype, device=dev) for w in (cache.dim, cache.vdim))
+    T, n, dev = q.shape[0], cu_seqlens.numel() - 1, q.device
+    data, sizes, place = _kv8_parts(cache)
+    k, v = (torch.empty(n * max_len, sizes[0], w, dtype=q.dtype, device=dev) for w in sizes[1:])
     rows = torch.empty(T, dtype=torch.int32, device=dev)
-    _check(lib().ell_kv8_read(*_kv8(cache), _p(k), _p(v), _p(base), _p(length), _p(cu_seqlens), _p(rows), c_int(n), c_int(T), c_int(max_len), *sizes, *place,
-                              _bf(q.dtype), _p(err_flag(dev)), _stream()), "kv8_read")
+    _check(_kv8_fn("ell_kv8_read")(*data, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(), rows.data_ptr(), n, T,
+                                   max_len, *sizes, *place, _is_bf(q.dtype), _err_word(dev), _stream()), "kv8_read")
     out = attention_rows(q, k, v, rows, length, max_len, scale, sink, alibi_slopes, window, None, cu_seqlens, max_q)
-    _check(lib().ell_kv8_clear(_p(out), _p(length), _p(cu_seqlens), c_int(n), c_int(T), c_int(out[0].numel()), _stream()), "kv8_clear")
+    _check(_kv8_fn("ell_kv8_clear")(out.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(), n, T, out.shape[1] * out.shape[2], _stream()), "kv8_clear")
     return out
 
 
-def attention_kv8(q, cache, base, length, max_len, scale, sink=None, alibi_slopes=None, window=None, cu_seqlens=None, max_q=None):
-    T, H, d = q.shape
+@_on_device
+def attention_kv8(q, cache, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):
+    (T, H, d), (data, sizes, place) = q.shape, _kv8_parts(cache)
+    G, _, dv = sizes
+    window = window or 0
     n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, max_q)
-    sizes, place = _kv8_sizes(cache)
-    G = cache.k.shape[1]
-    if max_q * (H // G) >= KV8_READ_ROWS and q.dtype == torch.bfloat16 and not ((d | cache.vdim) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4) and \
-            2 * n_seq * max_len * G * (d + cache.vdim) <= KV8_READ_BYTES:
-        with _on(q.device):
-            return _attention_read_back(q, cache, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
-    with _on(q.device):
-        out = torch.empty(T, H, cache.vdim, dtype=q.dtype, device=q.device)
-        sl = cu._slopes(alibi_slopes, H, q.device)
-        need = lib().ell_attn_kv8_scratch(c_int(T), c_int(n_seq), c_int(max_q), c_int(H), sizes[0], c_int(max_len), c_int(window or 0))
-        part = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
-        _check(lib().ell_attn_kv8(_p(q), *_kv8(cache), _p(out), _p(part), _p(base), _p(length), _p(None if sink is None else _f32(sink, "sink")), _p(sl),
-                                  _p(cu_seqlens), c_int(T), c_int(n_seq), c_int(max_q), c_int(H), *sizes, c_int(_heads(q, "q")), c_int(max_len),
-                                  c_int(window or 0), c_float(scale), *place, _bf(q.dtype), _p(err_flag(q.device)), _stream()), "attn_kv8", 2 if need else 1)
+    if max_q * (H // G) >= KV8_READ_ROWS and q.dtype is torch.bfloat16 and not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4) and \
+            2 * n_seq * max_len * G * (d + dv) <= KV8_READ_BYTES:
+        return _attention_read_back(q, cache, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
+    out = q.new_empty((T, H, dv))
+    # room for what shares cut (csrc/kv8.cu): a call has no more CTAs than are resident, or a CTA for each key head and 16 of its query heads
+    need = max(KV8_CTAS, G * -(-(H // G) // 16)) * KV8_CTA_FLOATS if max_len > KV8_UNCUT else 0
+    part = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+    sl = None if alibi_slopes is None else cu._slopes(alibi_slopes, H, q.device)
+    _check(_kv8_fn("ell_attn_kv8")(q.data_ptr(), *data, out.data_ptr(), None if part is None else part.data_ptr(), need, base.data_ptr(), length.data_ptr(),
+                                   None if sink is None else _f32(sink, "sink").data_ptr(), None if sl is None else sl.data_ptr(),
+                                   None if cu_seqlens is None else cu_seqlens.data_ptr(), T, n_seq, max_q, H, *sizes, _packed(q, "q"), max_len, window,
+                                   scale, *place, _is_bf(q.dtype), _err_word(q.device), _stream()), "attn_kv8", 2 if need else 1)
     return out
 
 

@@ -268,21 +268,19 @@ def kv8_empty(rows, heads, dim, vdim, block, device=None):
 
 
 def _kv8_check(cache, *ints):
+    """Raises where ``cache`` is not a ``KV8``, or an index vector not one; a serving step asks once a call, so it is put briefly."""
     k, v, ks, vs, d, dv = cache
-    R, G = k.shape[:2]
-    block = R // max(1, ks.shape[0])
-    if k.shape != (R, G, -(-d // 16) * 16) or v.shape != (R, G, -(-dv // 16) * 16) or k.dtype != torch.int8 or v.dtype != torch.int8 or \
-            not 1 <= min(d, dv) <= max(d, dv) <= KV8_MOST or ks.shape != vs.shape or ks.shape != (R // block if block else 0, G) or \
-            ks.shape[0] * block != R or not 1 <= block <= KV8_MOST or block & (block - 1) or ks.dtype != torch.float32 or vs.dtype != torch.float32 or \
-            not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+    (R, G, wk), (Rv, Gv, wv), (B, Gs), dev = k.shape, v.shape, ks.shape, k.get_device()
+    block = R // B if B else 0
+    if not (k.dtype is v.dtype is torch.int8 and ks.dtype is vs.dtype is torch.float32 and Rv == R and Gv == G == Gs and vs.shape == ks.shape and
+            0 < d <= wk <= KV8_MOST and 0 < dv <= wv <= KV8_MOST and wk == d + -d % 16 and wv == dv + -dv % 16 and B * block == R and
+            0 < block <= KV8_MOST and not block & (block - 1) and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("an 8-bit cache is contiguous: int8 [R, G, dim padded to 16] rows, fp32 [R / block, G] scales, blocks of a power of two")
-    for t in (v, ks, vs) + ints:
-        if t.device != k.device:
-            raise ValueError(f"8-bit cache on {k.device}, an operand on {t.device}")
+    if not dev == v.get_device() == ks.get_device() == vs.get_device():
+        raise ValueError("the parts of an 8-bit cache are on one device")
     for t in ints:
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
-            raise ValueError("places and lengths of cache rows are contiguous int32 vectors")
-    return block
+        if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.get_device() != dev:
+            raise ValueError("places and lengths of cache rows are contiguous int32 vectors on the cache's device")
 
 
 def kv8_append(cache, k, v, meta):
@@ -294,11 +292,11 @@ def kv8_append(cache, k, v, meta):
     base, length, cu = meta["kv_base"], meta["kv_len"], meta["cu_seqlens"]
     _kv8_check(cache, base, length, cu)
     T, G = k.shape[0], cache.k.shape[1]
-    if k.shape != (T, G, cache.dim) or v.shape != (T, G, cache.vdim) or k.dtype != v.dtype or k.device != cache.k.device or v.device != k.device or \
+    if k.shape != (T, G, cache.dim) or v.shape != (T, G, cache.vdim) or k.dtype != v.dtype or not k.get_device() == v.get_device() == base.get_device() or \
             base.numel() != T or length.numel() != T:
         raise ValueError(f"kv8_append: k [T, {G}, {cache.dim}] and v [T, {G}, {cache.vdim}] of one dtype, a place and a length for each row")
     if _kern(k):
-        return _cu().kv8_append(cache, k, v, base, length, cu, meta["max_seqlen"])
+        return _cu().kv8_append(k, v, cache, base, length, cu, meta["max_seqlen"])
     ref.kv8_append(cache, k, v, meta)
 
 
@@ -309,7 +307,7 @@ def kv8_read(cache, kv_base, kv_len, max_len, dtype=torch.bfloat16):
     if kv_base.shape != kv_len.shape or dtype not in (torch.bfloat16, torch.float32) or max_len < 0:
         raise ValueError("kv8_read: a place and a length for each sequence, into bf16 or fp32")
     if cache.k.is_cuda:
-        return _cu().kv8_read(cache, kv_base, kv_len, max_len, dtype)
+        return _cu().kv8_read(kv_base, kv_len, cache, max_len, dtype)
     return ref.kv8_read(cache, kv_base, kv_len, max_len, dtype)
 
 
@@ -322,13 +320,13 @@ def attention_kv8(q, cache, kv_base, kv_len, max_len, scale, sink=None, alibi_sl
     ints = (kv_base, kv_len) if cu_seqlens is None else (kv_base, kv_len, cu_seqlens)
     _kv8_check(cache, *ints)
     T, H, d = q.shape
-    if d != cache.dim or H % cache.k.shape[1] or q.device != cache.k.device or kv_base.numel() != T or kv_len.numel() != T:
+    if d != cache.dim or H % cache.k.shape[1] or q.get_device() != kv_base.get_device() or kv_base.numel() != T or kv_len.numel() != T:
         raise ValueError(f"attention_kv8: q [T, H, {cache.dim}] with a multiple of {cache.k.shape[1]} heads, a place and a length for each row")
     if window is not None and window < 1:
         raise ValueError(f"attention_kv8: a window of {window} rows")
     for t, name in ((sink, "sink"), (alibi_slopes, "alibi_slopes")):
-        if t is not None and t.numel() != H:
-            raise ValueError(f"attention_kv8: {name} has one value for each of the {H} heads, got {t.numel()}")
+        if t is not None and (t.numel() != H or t.get_device() != q.get_device()):
+            raise ValueError(f"attention_kv8: {name} has one value for each of the {H} heads on their device")
     if cu_seqlens is not None and max_q is None:
         raise ValueError("attention_kv8: cu_seqlens comes with max_q, a bound of the sequences' rows")
     if _kern(q):
