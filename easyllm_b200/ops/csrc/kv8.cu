@@ -698,9 +698,8 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   const int hg = blockIdx.x % hs, share = blockIdx.x / hs, g = hg / groups, h0 = g * rep + hg % groups * kK8Heads, nh = min(kK8Heads, (g + 1) * rep - h0);
   int x = share, q0 = 0, left = 0x7fffffff, all = 0, shares = 1;
   if (a.cut) {
-    // where the share begins: a thread counts the quanta of its tiles, and walks them if it is there
-    int* found = reinterpret_cast<int*>(sm);           // sums of the warps | tile, quanta before the share's first in it
-    const int chunk = (n_x + kK8Threads - 1) / kK8Threads, first = min((int)threadIdx.x * chunk, n_x), last = min(first + chunk, n_x);
+    // where the share begins: a lane counts the quanta of its tiles, and walks them if it is there; every warp for itself, without a barrier
+    const int chunk = (n_x + 31) / 32, first = min(lane * chunk, n_x), last = min(first + chunk, n_x);
     int mine = 0;
     for (int i = first; i < last; ++i) mine += K8Tile(a, i).quanta();
     int before = mine;
@@ -709,35 +708,26 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       const int y = __shfl_up_sync(0xffffffffu, before, o);
       if (lane >= o) before += y;
     }
-    if (lane == 31) found[warp] = before;
+    all = __shfl_sync(0xffffffffu, before, 31);
     before -= mine;
-    __syncthreads();
-    int total = 0;
-    for (int w = 0; w < 4; ++w) {
-      if (w == warp) before += total;
-      total += found[w];
-    }
-    all = total;
-    shares = max(1, min((int)gridDim.x / hs, total));  // none is empty
-    const int begin = (int)((long long)share * total / shares);
-    left = share < shares ? (int)((share + 1ll) * total / shares) - begin : 0;
-    if (left > 0 && begin >= before && begin < before + mine) {
-      int at = begin - before, i = first;
-      for (; i < last - 1; ++i) {
-        const int q = K8Tile(a, i).quanta();
-        if (at < q) break;
-        at -= q;
-      }
-      found[4] = i;
-      found[5] = at;
-    }
+    shares = max(1, min((int)gridDim.x / hs, all));    // none is empty
+    const int begin = (int)((long long)share * all / shares);
+    left = share < shares ? (int)((share + 1ll) * all / shares) - begin : 0;
     if (threadIdx.x == 0) reinterpret_cast<K8Cut*>(a.part + (size_t)gridDim.x * 2 * R * LD)[blockIdx.x].more = 0;
-    __syncthreads();
     if (left == 0) return;
-    x = found[4];
-    q0 = found[5];
-    sm100::fence_proxy_async_smem();
-    __syncthreads();
+    const bool here = begin >= before && begin < before + mine;
+    x = first;
+    q0 = begin - before;
+    if (here) {
+      for (; x < last - 1; ++x) {
+        const int q = K8Tile(a, x).quanta();
+        if (q0 < q) break;
+        q0 -= q;
+      }
+    }
+    const int who = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    x = __shfl_sync(0xffffffffu, x, who);
+    q0 = __shfl_sync(0xffffffffu, q0, who);
   }
   uint8_t* stages = sm + warp * kK8Stage * kStages;
   volatile int* gave_up = &ring.gave_up;
@@ -932,58 +922,67 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 }
 
 // Joins the pieces of the items that shares cut.  A CTA the item that begins in the share (and heads) of its number, if that one was cut.
-// A row has 32 / R warps, each with its share of the pieces: one long sequence has some fifty of them for a few rows, whose loads are to be under
-// way together (a warp a row took 22 us there).
-constexpr int kK8JoinThreads = 1024;
+// A row has W warps, each with every W-th piece, eight of which are under way together: one long sequence has some fifty.  The CTAs are
+// small enough to be resident all at once, most of them have nothing to do (as CTAs of 1024 threads, in three rounds, they took 12 us).
+constexpr int kK8JoinThreads = 512;
 template <typename T, int R>
-__global__ void __launch_bounds__(kK8JoinThreads) attn_kv8_join_kernel(const __grid_constant__ Kv8Attn a) {
+__global__ void __launch_bounds__(kK8JoinThreads, 2) attn_kv8_join_kernel(const __grid_constant__ Kv8Attn a) {
   chain_enter();
   constexpr int W = kK8JoinThreads / 32 / R;
   __shared__ float4 sums[W][R][32];
-  __shared__ float stat[W][R];
+  __shared__ float2 stat[W][R];
   const int hs = k8_groups(a.H, a.c.G);
   const K8Cut cut = reinterpret_cast<const K8Cut*>(a.part + (size_t)gridDim.x * 2 * R * kK8SlotRow)[blockIdx.x];
-  const int m = (threadIdx.x >> 5) % R, part = (threadIdx.x >> 5) / R, lane = threadIdx.x & 31;
+  const int m = (threadIdx.x >> 5) % R, mine = (threadIdx.x >> 5) / R, lane = threadIdx.x & 31;
   if (cut.more == 0) return;
   const int pieces = cut.more + 1, h = cut.h0 + m % cut.nh;
-  auto slot = [&](int i) { return a.part + ((size_t)(blockIdx.x + i * hs) * 2 + (i == 0)) * R * kK8SlotRow + m * kK8SlotRow; };
+  const float* const slots = a.part + m * kK8SlotRow;
   if (m < cut.rows) {
-    float mx = -INFINITY;
-    for (int i = lane; i < pieces; i += 32) mx = fmaxf(mx, slot(i)[kK8Dim]);
-    const float sk = a.sink != nullptr ? a.sink[h] * kLog2e : -INFINITY, top = fmaxf(warp_max(mx), sk), ref = top == -INFINITY ? 0.f : top;
-    float l = part == 0 && lane == 0 ? exp2f(sk - ref) : 0.f;
+    const float sk = mine == 0 && a.sink != nullptr ? a.sink[h] * kLog2e : -INFINITY;
+    float top = sk, l = sk == -INFINITY ? 0.f : 1.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = part; i0 < pieces; i0 += W * 8) {
+    for (int i0 = mine; i0 < pieces; i0 += W * 8) {
       float4 v[8];
-      float w[8], x[8];
+      float2 st[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float* s = slot(min(i0 + W * i, pieces - 1));
+        const int at = min(i0 + W * i, pieces - 1);
+        const float* s = slots + ((size_t)(blockIdx.x + at * hs) * 2 + (at == 0)) * R * kK8SlotRow;
         v[i] = *reinterpret_cast<const float4*>(s + 4 * lane);
-        w[i] = i0 + W * i < pieces ? s[kK8Dim] : -INFINITY;
-        x[i] = s[kK8Dim + 1];
+        st[i] = *reinterpret_cast<const float2*>(s + kK8Dim);
       }
+      float now = top;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) now = fmaxf(now, st[i].x);
+      const float ref = now == -INFINITY ? 0.f : now, al = exp2f(top - ref);
+      top = now;
+      l *= al;
+      o = make_float4(o.x * al, o.y * al, o.z * al, o.w * al);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const bool is = i0 + W * i < pieces;           // the last one again has no part
-        const float e = exp2f(w[i] - ref);
-        if (!is) continue;
-        o = make_float4(fmaf(v[i].x, e, o.x), fmaf(v[i].y, e, o.y), fmaf(v[i].z, e, o.z), fmaf(v[i].w, e, o.w));
-        if (lane == 0) l = fmaf(x[i], e, l);
+        if (i0 + W * i < pieces) {
+          const float e = exp2f(st[i].x - ref);
+          l = fmaf(st[i].y, e, l);
+          o = make_float4(fmaf(v[i].x, e, o.x), fmaf(v[i].y, e, o.y), fmaf(v[i].z, e, o.z), fmaf(v[i].w, e, o.w));
+        }
       }
     }
-    sums[part][m][lane] = o;
-    if (lane == 0) stat[part][m] = l;
+    sums[mine][m][lane] = o;
+    if (lane == 0) stat[mine][m] = make_float2(top, l);
   }
   __syncthreads();
-  if (m >= cut.rows || part != 0) return;
-  float4 o = sums[0][m][lane];
-  float den = stat[0][m];
+  if (m >= cut.rows || mine != 0) return;
+  float top = stat[0][m].x, den = 0.f;
 #pragma unroll
-  for (int y = 1; y < W; ++y) {
+  for (int y = 1; y < W; ++y) top = fmaxf(top, stat[y][m].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int y = 0; y < W; ++y) {
     const float4 v = sums[y][m][lane];
-    o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
-    den += stat[y][m];
+    const float e = exp2f(stat[y][m].x - ref);
+    o = make_float4(fmaf(v.x, e, o.x), fmaf(v.y, e, o.y), fmaf(v.z, e, o.z), fmaf(v.w, e, o.w));
+    den = fmaf(stat[y][m].y, e, den);
   }
   const float f = den == 0.f ? 0.f : 1.f / den;
   k8_store_row<T>(a, cut.r0 + m / cut.nh, h, lane, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
