@@ -396,6 +396,10 @@ __device__ __forceinline__ int k8_next(const Kv8Attn& a, int n_x, int x) {
     if (a.cu == nullptr || a.cu[x / a.tiles] + x % a.tiles * a.tt < min(a.cu[x / a.tiles + 1], a.n)) break;
   return x;
 }
+// Where share i of n begins among `all` quanta.
+__device__ __forceinline__ int k8_share(int i, int all, int n) {
+  return all < (1 << 20) ? (int)((unsigned)i * (unsigned)all / (unsigned)n) : (int)((long long)i * all / n);      // i is below 2^12 then, as the CTAs are
+}
 // What the joining kernel needs to know of an item that begins in a CTA's share and is cut by its end.
 struct K8Cut {
   int r0, rows, h0, nh, more;     // more: shares after this one that have a piece of it (0: nothing was cut)
@@ -459,24 +463,40 @@ __device__ __forceinline__ void transpose_bytes(uint32_t a, uint32_t b, uint32_t
   y[3] = __byte_perm(ab1, cd1, 0x7632);
 }
 
-// The 32 elements 32 c .. 32 c + 31 of a row of `d`.
+// The 32 elements 32 c .. 32 c + 31 of a query row, as they come, with what else a row of queries needs from memory: all of it is asked for before any
+// of it is looked at.
 template <typename T>
-__device__ __forceinline__ void k8_load_query(const T* src, int c, int d, bool vec, float (&f)[32]) {
+struct K8Query {
+  static constexpr int kWords = 8 * sizeof(T);         // of 32 elements
+  uint32_t u[kWords];
+  float slope;
+  int end;
+  __device__ __forceinline__ void load(const Kv8Attn& a, int tok, int h, int c) {
+    const T* src = reinterpret_cast<const T*>(a.q) + (size_t)tok * a.ldq + (size_t)h * a.c.d + 32 * c;
+    const int d = a.c.d - 32 * c;
+    if (a.c.d % 8 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 8) {
-    const int at = 32 * c + i;
-    float g[8];
-    if (vec && at < d) {                                // d a multiple of 8
-      load_v<8>(src + at, g);
+      for (int i = 0; i < kWords; i += 4) {
+        const bool in = i * 4 / (int)sizeof(T) < d;
+        const uint4 w = in ? *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(src) + i) : make_uint4(0, 0, 0, 0);
+        u[i] = w.x, u[i + 1] = w.y, u[i + 2] = w.z, u[i + 3] = w.w;
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] = at + e < d ? to_f<T>(src[at + e]) : 0.f;
+      for (int i = 0; i < 32; ++i) {
+        const float f = i < d ? to_f<T>(src[i]) : 0.f;
+        if (sizeof(T) == 4) u[i % kWords] = __float_as_uint(f);
+        else u[i / 2 % kWords] = i & 1 ? u[i / 2 % kWords] | (__float_as_uint(f) & 0xffff0000u) : __float_as_uint(f) >> 16;
+      }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[i + e] = g[e];
+    end = a.len[tok];
+    slope = a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
   }
-}
-
+  __device__ __forceinline__ float at(int i) const {
+    if (sizeof(T) == 4) return __uint_as_float(u[i % kWords]);
+    return __uint_as_float(i & 1 ? u[i / 2 % kWords] & 0xffff0000u : u[i / 2 % kWords] << 16);
+  }
+};
 // What a warp keeps of a group of 8 rows; lane (g, c) has row g.
 struct K8Rows {
   uint32_t q[4][4], high[4][2];   // bytes of the query, of 32 columns each: low and middle as an operand, high
@@ -485,13 +505,10 @@ struct K8Rows {
   int first, end;                 // keys the row sees
 };
 template <typename T>
-__device__ __forceinline__ void k8_load_rows(const Kv8Attn& a, int tok, int h, int c, K8Rows& r) {
-  const T* src = reinterpret_cast<const T*>(a.q) + (size_t)tok * a.ldq + (size_t)h * a.c.d;
-  const bool vec = a.c.d % 8 == 0 && (reinterpret_cast<uintptr_t>(src) & (8 * sizeof(T) > 16 ? 15 : 8 * sizeof(T) - 1)) == 0;
-  float f[32], big = 0.f;
-  k8_load_query<T>(src, c, a.c.d, vec, f);
+__device__ __forceinline__ void k8_rows(const Kv8Attn& a, const K8Query<T>& f, K8Rows& r) {
+  float big = 0.f;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) big = max_nan(big, fabsf(f[i]));
+  for (int i = 0; i < 32; i += 2) big = max3_nan(big, fabsf(f.at(i)), fabsf(f.at(i + 1)));
   big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 1));
   big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 2));
   const int e = max((int)(__float_as_uint(big) >> 23), 1);            // biased exponent
@@ -504,15 +521,15 @@ __device__ __forceinline__ void k8_load_rows(const Kv8Attn& a, int tok, int h, i
     for (int x = 0; x < 2; ++x) {
       uint32_t v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = (__float_as_uint(fmaf(f[8 * s + 4 * x + i] * inv, 2097152.f, kMagicF)) - kMagic + 0x808080u) ^ 0x808080u;
+      for (int i = 0; i < 4; ++i) v[i] = (__float_as_uint(fmaf(f.at(8 * s + 4 * x + i) * inv, 2097152.f, kMagicF)) - kMagic + 0x808080u) ^ 0x808080u;
       const uint32_t ab = __byte_perm(v[0], v[1], 0x5140), cd = __byte_perm(v[2], v[3], 0x5140);
       r.q[s][2 * x] = __byte_perm(ab, cd, 0x5410);
       r.q[s][2 * x + 1] = __byte_perm(ab, cd, 0x7632);
       r.high[s][x] = __byte_perm(__byte_perm(v[0], v[1], 0x0062), __byte_perm(v[2], v[3], 0x0062), 0x5410);
     }
-  r.end = a.len[tok];
+  r.end = f.end;
   r.first = max(0, r.end - a.window);
-  r.slope = a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
+  r.slope = f.slope;
   r.m = -INFINITY;
   r.l = 0.f;
 }
@@ -711,8 +728,8 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     all = __shfl_sync(0xffffffffu, before, 31);
     before -= mine;
     shares = max(1, min((int)gridDim.x / hs, all));    // none is empty
-    const int begin = (int)((long long)share * all / shares);
-    left = share < shares ? (int)((share + 1ll) * all / shares) - begin : 0;
+    const int begin = k8_share(share, all, shares);
+    left = share < shares ? k8_share(share + 1, all, shares) - begin : 0;
     if (threadIdx.x == 0) reinterpret_cast<K8Cut*>(a.part + (size_t)gridDim.x * 2 * R * LD)[blockIdx.x].more = 0;
     if (left == 0) return;
     const bool here = begin >= before && begin < before + mine;
@@ -775,13 +792,13 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       fresh = false;
     }
     left -= p.q1 - p.q0;
-    const int x1 = left > 0 && a.cut ? k8_next(a, n_x, x) : n_x;
-    const bool more = x1 < n_x;
     send(kStages);
-    if (more) {                                        // the next piece, for the copies
-      const K8Piece n(a, x1, 0, left);
-      n_units = n.units(warp);
-      n_row = n.t.base + n.k0() + warp * kK8Keys;
+    // queries, scales and the next piece: what they need comes from memory together
+    K8Query<T> query[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int m = min(b * 8 + gr, rows - 1);         // rows past the end repeat the last
+      query[b].load(a, p.t.r0 + m / nh, h0 + m % nh, c);
     }
     float kn[2], vn[2];                                // scales of keys `lane` and lane + 32 of the next unit
     auto load_scales = [&](int i) {
@@ -795,13 +812,19 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       }
     };
     load_scales(0);
+    const int x1 = left > 0 && a.cut ? k8_next(a, n_x, x) : n_x;
+    const bool more = x1 < n_x;
+    if (more) {                                        // the next piece, for the copies
+      const K8Piece n(a, x1, 0, left);
+      n_units = n.units(warp);
+      n_row = n.t.base + n.k0() + warp * kK8Keys;
+    }
     K8Rows r[NB];
     float2 acc[NB][16];
     uint32_t q_high[4][4];                             // high bytes of the first group, and of the second or nothing
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int m = min(b * 8 + gr, rows - 1);         // rows past the end repeat the last
-      k8_load_rows<T>(a, p.t.r0 + m / nh, h0 + m % nh, c, r[b]);
+      k8_rows<T>(a, query[b], r[b]);
 #pragma unroll
       for (int y = 0; y < 16; ++y) acc[b][y] = make_float2(0.f, 0.f);
     }
@@ -866,7 +889,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     const bool whole = began == 0 && behind == 0;
     float* slot = whole ? nullptr : a.part + ((size_t)blockIdx.x * 2 + (began == 0)) * R * LD;
     if (!whole && began == 0 && threadIdx.x == 0) {    // its last quantum is the share's of which the first is not behind it
-      const long long last = (share + 1ll) * all / shares + behind - 1;
+      const long long last = k8_share(share + 1, all, shares) + behind - 1ll;
       reinterpret_cast<K8Cut*>(a.part + (size_t)gridDim.x * 2 * R * LD)[blockIdx.x] = K8Cut{r0, n_rows, h0, nh, (int)(((last + 1) * shares - 1) / all) - share};
     }
     const float* from[4];
