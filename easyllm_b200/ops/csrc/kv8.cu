@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Cache c, T* __re
   if (cu != nullptr) {
     r0 = cu[i];
     r1 = min(cu[i + 1], rows);
-    if (r0 >= r1) return;
+    if (r0 < 0 || r0 >= r1) return;
     if (blockIdx.x == 0)
       for (int r = r0 + threadIdx.x; r < r1; r += 256) row_base[r] = i * max_len;
   }
@@ -366,6 +366,7 @@ struct K8Tile {
       r1 = min(r0 + a.tt, end);
     }
     len0 = len1 = low = base = 0;
+    if (r0 < 0) r1 = r0;
     if (r0 >= r1) return;
     len0 = a.len[r0];
     len1 = a.len[r1 - 1];
@@ -393,7 +394,7 @@ struct K8Piece {
 // The next tile with rows, or n_x.
 __device__ __forceinline__ int k8_next(const Kv8Attn& a, int n_x, int x) {
   while (++x < n_x)
-    if (a.cu == nullptr || a.cu[x / a.tiles] + x % a.tiles * a.tt < min(a.cu[x / a.tiles + 1], a.n)) break;
+    if (a.cu == nullptr || (a.cu[x / a.tiles] >= 0 && a.cu[x / a.tiles] + x % a.tiles * a.tt < min(a.cu[x / a.tiles + 1], a.n))) break;
   return x;
 }
 // Where share i of n begins among `all` quanta.
@@ -1046,49 +1047,89 @@ static int launch_attn_kv8(const Kv8Attn& a, const K8Plan& p, const CUtensorMap&
   return launch_status();
 }
 
-static bool k8_sizes_ok(int G, int d, int dv, int shift) {
-  return G > 0 && d > 0 && dv > 0 && d <= kK8Dim && dv <= kK8Dim && shift >= 0 && (1 << shift) <= kK8MaxBlock;
-}
-
 }  // namespace ell
 
 using namespace ell;
 
+// The arguments come as structures of 64-bit words: from Python thirty words of one object cost less than thirty arguments.
+struct Kv8Args {                  // a cache: rows, scales, heads and head sizes, rows that share a scale, rows in all
+  int8_t *k, *v;
+  float *ks, *vs;
+  long long G, d, dv, block, rows;
+};
+struct Kv8AppendCall {
+  Kv8Args c;
+  const void *k, *v;
+  const int *base, *len, *cu;
+  long long n, n_seq, max_new, ldk, ldv, is_bf16;
+  int* err;
+};
+struct Kv8ReadCall {
+  Kv8Args c;
+  void *k, *v;
+  const int *base, *len, *cu;
+  int* row_base;
+  long long n, rows_q, max_len, is_bf16;
+  int* err;
+};
+struct Kv8AttnCall {
+  Kv8Args c;
+  const void* q;
+  void* out;
+  float* part;
+  long long part_floats;
+  const int *base, *len;
+  const float *sink, *slopes;
+  const int* cu;
+  long long n, n_seq, max_q, H, ldq, max_len, window, is_bf16;
+  int* err;
+  double scale;
+};
+static bool k8_cache(const Kv8Args& a, Kv8Cache& c) {
+  const bool ok = a.G > 0 && a.G <= 65535 && a.d > 0 && a.dv > 0 && a.d <= kK8Dim && a.dv <= kK8Dim && a.block > 0 && a.block <= kK8MaxBlock &&
+                  !(a.block & (a.block - 1)) && a.rows % a.block == 0 && a.rows <= 0x7fffffff;
+  int shift = 0;
+  while ((1ll << shift) < a.block) ++shift;
+  c = Kv8Cache{a.k, a.v, a.ks, a.vs, a.rows, (int)a.G, (int)a.d, (int)a.dv, shift};
+  return ok;
+}
+
 // The rows k [n, G, d], v [n, G, dv] (rows of ldk / ldv elements) of a step: those of cu[i] .. cu[i + 1] - 1 go to the places
 // len[cu[i]] - 1 and on of the sequence whose rows start at base[cu[i]].  max_new bounds their number.
-ELL_API int ell_kv8_append(int8_t* kc, int8_t* vc, float* ks, float* vs, const void* k, const void* v, const int* base, const int* len, const int* cu,
-                           int n, int n_seq, int max_new, int G, int d, int dv, int ldk, int ldv, int shift, long long rows, int is_bf16, int* err,
-                           cudaStream_t stream) {
-  if (n <= 0 || n_seq <= 0 || max_new <= 0) return 0;
-  if (!k8_sizes_ok(G, d, dv, shift)) return -2;
-  const Kv8Cache c{kc, vc, ks, vs, rows, G, d, dv, shift};
-  const int block = 1 << shift, esz = is_bf16 ? 2 : 4;
-  const long long blocks = ((long long)max_new + 2 * block - 2) / block, ctas = ((long long)n_seq * blocks * 2 * G + 7) / 8;
+ELL_API int ell_kv8_append(const Kv8AppendCall* call, cudaStream_t stream) {
+  const Kv8AppendCall& x = *call;
+  Kv8Cache c;
+  if (x.n <= 0 || x.n_seq <= 0 || x.max_new <= 0) return 0;
+  if (!k8_cache(x.c, c) || x.n > 0x7fffffff) return -2;
+  const int esz = x.is_bf16 ? 2 : 4;
+  const long long blocks = (x.max_new + 2 * x.c.block - 2) / x.c.block, ctas = (x.n_seq * blocks * 2 * c.G + 7) / 8;
   if (ctas > 0x0fffffff) return -2;
-  const bool vec = d % 8 == 0 && dv % 8 == 0 && ldk * esz % 16 == 0 && ldv * esz % 16 == 0 && aligned_to(k, 16) && aligned_to(v, 16);
-#define ELL_APPEND(T, V)                                                                                                                                   \
-  launch_chained(kv8_append_kernel<T, V>, (unsigned)ctas, 256, 0, stream, c, (const T*)k, (const T*)v, base, len, cu, n_seq, n, (int)blocks, ldk, ldv, err)
-  if (is_bf16) vec ? ELL_APPEND(__nv_bfloat16, 8) : ELL_APPEND(__nv_bfloat16, 1);
+  const bool vec = c.d % 8 == 0 && c.dv % 8 == 0 && x.ldk * esz % 16 == 0 && x.ldv * esz % 16 == 0 && aligned_to(x.k, 16) && aligned_to(x.v, 16);
+#define ELL_APPEND(T, V)                                                                                                                              \
+  launch_chained(kv8_append_kernel<T, V>, (unsigned)ctas, 256, 0, stream, c, (const T*)x.k, (const T*)x.v, x.base, x.len, x.cu, (int)x.n_seq,          \
+                 (int)x.n, (int)blocks, (int)x.ldk, (int)x.ldv, x.err)
+  if (x.is_bf16) vec ? ELL_APPEND(__nv_bfloat16, 8) : ELL_APPEND(__nv_bfloat16, 1);
   else vec ? ELL_APPEND(float, 8) : ELL_APPEND(float, 1);
 #undef ELL_APPEND
   return launch_status();
 }
 
 // cu [n + 1] and row_base [rows_q] (or null, null): see kv8_read_kernel.
-ELL_API int ell_kv8_read(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, void* ko, void* vo, const int* base, const int* len,
-                         const int* cu, int* row_base, int n, int rows_q, int max_len, int G, int d, int dv, int shift, long long rows, int is_bf16, int* err,
-                         cudaStream_t stream) {
-  if (n <= 0 || max_len <= 0) return 0;
-  if (!k8_sizes_ok(G, d, dv, shift) || n > 65535 || (cu != nullptr && (long long)n * max_len > 0x7fffffff)) return -2;
-  const Kv8Cache c{const_cast<int8_t*>(kc), const_cast<int8_t*>(vc), const_cast<float*>(ks), const_cast<float*>(vs), rows, G, d, dv, shift};
-  const int vec = d % 8 == 0 && dv % 8 == 0 ? 8 : 1;
+ELL_API int ell_kv8_read(const Kv8ReadCall* call, cudaStream_t stream) {
+  const Kv8ReadCall& x = *call;
+  Kv8Cache c;
+  if (x.n <= 0 || x.max_len <= 0) return 0;
+  if (!k8_cache(x.c, c) || x.n > 65535 || x.max_len > 0x3fffffff || (x.cu != nullptr && x.n * x.max_len > 0x7fffffff)) return -2;
+  const int vec = c.d % 8 == 0 && c.dv % 8 == 0 ? 8 : 1;
   // positions of a CTA: sixteen turns of its threads, fewer where that leaves SMs without work
-  const int per = G * (d + dv) / vec, beside = std::max(1, 256 / per);
-  const long long most = (long long)n * max_len / (8 * kNumSMs) + 1;
+  const int per = c.G * (c.d + c.dv) / vec, beside = std::max(1, 256 / per);
+  const long long most = x.n * x.max_len / (8 * kNumSMs) + 1;
   const int chunk = (int)std::max<long long>(beside, std::min<long long>(16 * beside, most / beside * beside));
-  const dim3 grid((max_len + chunk - 1) / chunk, n);
-#define ELL_READ(T, V) launch_chained(kv8_read_kernel<T, V>, grid, 256, 0, stream, c, (T*)ko, (T*)vo, base, len, cu, row_base, rows_q, max_len, chunk, err)
-  if (is_bf16) vec == 8 ? ELL_READ(__nv_bfloat16, 8) : ELL_READ(__nv_bfloat16, 1);
+  const dim3 grid((unsigned)((x.max_len + chunk - 1) / chunk), (unsigned)x.n);
+#define ELL_READ(T, V)                                                                                                                             \
+  launch_chained(kv8_read_kernel<T, V>, grid, 256, 0, stream, c, (T*)x.k, (T*)x.v, x.base, x.len, x.cu, x.row_base, (int)x.rows_q, (int)x.max_len, chunk, \
+                 x.err)
+  if (x.is_bf16) vec == 8 ? ELL_READ(__nv_bfloat16, 8) : ELL_READ(__nv_bfloat16, 1);
   else vec == 8 ? ELL_READ(float, 8) : ELL_READ(float, 1);
 #undef ELL_READ
   return launch_status();
@@ -1104,23 +1145,22 @@ ELL_API int ell_kv8_clear(void* out, const int* len, const int* cu, int n_seq, i
 // q rows of ldq elements.  max_len bounds len[].  part (16-byte aligned): `part_floats` of scratch where max_len is above 256, enough for
 // max(444, key heads x groups of 16 query heads) x 4232.  window: keys a row sees (<= 0: all).  cu [n_seq + 1] (or null): rows
 // cu[i] .. cu[i + 1] - 1 are consecutive tokens of one sequence, with one base and lengths that grow by one; max_q bounds their number.
-ELL_API int ell_attn_kv8(const void* q, const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, void* out, float* part, long long part_floats,
-                         const int* base, const int* len, const float* sink, const float* slopes, const int* cu, int n, int n_seq, int max_q, int H, int G, int d, int dv,
-                         int ldq, int max_len, int window, float scale, int shift, long long rows, int is_bf16, int* err, cudaStream_t stream) {
-  if (n <= 0) return 0;
-  if (!k8_sizes_ok(G, d, dv, shift) || H % G || rows > 0x7fffffff) return -2;
-  if (cu == nullptr) n_seq = 0;
-  const K8Plan p = k8_plan(n, n_seq, max_q, H, G, max_len, window);
-  if (p.cut && (part == nullptr || !aligned_to(part, 16) || (size_t)part_floats < k8_part_floats(p))) return -2;
+ELL_API int ell_attn_kv8(const Kv8AttnCall* call, cudaStream_t stream) {
+  const Kv8AttnCall& x = *call;
   Kv8Attn a{};
-  a.c = Kv8Cache{const_cast<int8_t*>(kc), const_cast<int8_t*>(vc), const_cast<float*>(ks), const_cast<float*>(vs), rows, G, d, dv, shift};
-  a.q = q, a.out = out, a.part = part, a.base = base, a.len = len, a.cu = cu, a.sink = sink, a.slopes = slopes;
-  a.n = n, a.H = H, a.ldq = ldq, a.n_seq = n_seq, a.tiles = p.tiles, a.tt = p.tt, a.cut = p.cut;
-  a.window = window > 0 ? window : 0x3fffffff, a.scale = (float)((double)scale * 1.4426950408889634 / 2097152), a.err = err;
+  if (x.n <= 0) return 0;
+  if (!k8_cache(x.c, a.c) || x.n > 0x7fffffff || x.H <= 0 || x.H > 0x7fffff || x.H % x.c.G || x.max_len > 0x3fffffff || x.max_q > 0x3fffffff) return -2;
+  const int n_seq = x.cu == nullptr ? 0 : (int)x.n_seq;
+  const K8Plan p = k8_plan((int)x.n, n_seq, (int)x.max_q, (int)x.H, a.c.G, (int)x.max_len, (int)std::min(x.window, 0x3fffffffll));
+  if (p.ctas <= 0) return -2;
+  if (p.cut && (x.part == nullptr || !aligned_to(x.part, 16) || (size_t)x.part_floats < k8_part_floats(p))) return -2;
+  a.q = x.q, a.out = x.out, a.part = x.part, a.base = x.base, a.len = x.len, a.cu = x.cu, a.sink = x.sink, a.slopes = x.slopes;
+  a.n = (int)x.n, a.H = (int)x.H, a.ldq = (int)x.ldq, a.n_seq = n_seq, a.tiles = p.tiles, a.tt = p.tt, a.cut = p.cut;
+  a.window = x.window > 0 ? (int)std::min(x.window, 0x3fffffffll) : 0x3fffffff, a.scale = (float)(x.scale * 1.4426950408889634 / 2097152), a.err = x.err;
   CUtensorMap tk, tv;
-  int rc = make_tmap_bytes_heads(&tk, kc, k8_row(d), G, rows, kK8Keys);
-  if (!rc) rc = make_tmap_bytes_heads(&tv, vc, k8_row(dv), G, rows, kK8Keys);
+  int rc = make_tmap_bytes_heads(&tk, a.c.k, k8_row(a.c.d), a.c.G, a.c.rows, kK8Keys);
+  if (!rc) rc = make_tmap_bytes_heads(&tv, a.c.v, k8_row(a.c.dv), a.c.G, a.c.rows, kK8Keys);
   if (rc) return rc;
-  if (is_bf16) return p.nb == 1 ? launch_attn_kv8<__nv_bfloat16, 1>(a, p, tk, tv, stream) : launch_attn_kv8<__nv_bfloat16, 2>(a, p, tk, tv, stream);
+  if (x.is_bf16) return p.nb == 1 ? launch_attn_kv8<__nv_bfloat16, 1>(a, p, tk, tv, stream) : launch_attn_kv8<__nv_bfloat16, 2>(a, p, tk, tv, stream);
   return p.nb == 1 ? launch_attn_kv8<float, 1>(a, p, tk, tv, stream) : launch_attn_kv8<float, 2>(a, p, tk, tv, stream);
 }

@@ -3,7 +3,8 @@ and the tcgen05 GEMM / attention) for bf16 and fp32 CUDA tensors; the signatures
 from __future__ import annotations
 
 import functools
-from ctypes import addressof, c_float, c_int, c_longlong, c_void_p
+import struct
+from ctypes import addressof, c_char_p, c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -281,20 +282,18 @@ def attention_rows(q, k, v, base, length, max_len, scale, sink=None, alibi_slope
 
 # ---- a cache held in 8 bits ------------------------------------------------------------------------
 # A decoding step calls these for every layer, and a short context's kernels take less time than a call from Python: the arguments go over
-# as numbers (a ctypes object each costs 0.2 us), types are declared once.
-_KV8_TYPES = {
-    "ell_kv8_append": "pppp pp ppp iii iii ii il i pp", "ell_kv8_read": "pppp pp pp pp iii iii il i pp", "ell_kv8_clear": "p pp iii p",
-    "ell_attn_kv8": "p pppp pp l pp pp p iii i iii i ii f il i pp"}
+# as the words of one structure (csrc/kv8.cu), nine of which are the cache's.
+_KV8_CALLS = {"ell_kv8_append": struct.Struct("9q 5q 7q").pack, "ell_kv8_read": struct.Struct("9q 6q 5q").pack, "ell_attn_kv8": struct.Struct("9q 9q 9q d").pack}
 _KV8_FNS, _ERR_WORDS = {}, {}
 
 
-def _kv8_fn(name):
+def _kv8_call(name, label, launches, *words):
     f = _KV8_FNS.get(name)
     if f is None:
         f = getattr(lib(), name)
-        f.argtypes = [{"p": c_void_p, "i": c_int, "l": c_longlong, "f": c_float}[t] for t in _KV8_TYPES[name].replace(" ", "")]
+        f.argtypes = [c_char_p, c_void_p]
         _KV8_FNS[name] = f
-    return f
+    _check(f(_KV8_CALLS[name](*words), _stream()), label, launches)
 
 
 def _err_word(device):
@@ -315,13 +314,6 @@ def _on_device(f):
     return call
 
 
-def _kv8_parts(cache):
-    """Arguments: addresses | heads, sizes | rows of a block as a shift, rows."""
-    k, v, ks, vs, d, dv = cache
-    R, G = k.shape[0], k.shape[1]
-    return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()), (G, d, dv), ((R // ks.shape[0]).bit_length() - 1, R)
-
-
 def _packed(t, name):
     """``_heads``, in fewer steps."""
     (T, H, d), (ld, heads, one) = t.shape, t.stride()
@@ -335,21 +327,18 @@ def _is_bf(dtype):
 
 
 @_on_device
-def kv8_append(k, v, cache, base, length, cu_seqlens, max_new):
-    data, sizes, place = _kv8_parts(cache)
-    _check(_kv8_fn("ell_kv8_append")(*data, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(), k.shape[0],
-                                     cu_seqlens.numel() - 1, max_new, *sizes, _packed(k, "k"), _packed(v, "v"), *place, _is_bf(k.dtype),
-                                     _err_word(k.device), _stream()), "kv8_append")
+def kv8_append(k, v, words, base, length, cu_seqlens, max_new):
+    _kv8_call("ell_kv8_append", "kv8_append", 1, *words, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(), k.shape[0],
+              cu_seqlens.numel() - 1, max_new, _packed(k, "k"), _packed(v, "v"), _is_bf(k.dtype), _err_word(k.device))
 
 
 @_on_device
-def kv8_read(base, length, cache, max_len, dtype):
-    n, (data, sizes, place) = base.numel(), _kv8_parts(cache)
-    G, d, dv = sizes
-    k = torch.empty((n, max_len, G, d), dtype=dtype, device=base.device)
+def kv8_read(base, length, words, max_len, dtype):
+    n, G, d, dv, dev = base.numel(), words[4], words[5], words[6], base.device
+    k = torch.empty((n, max_len, G, d), dtype=dtype, device=dev)
     v = torch.empty_like(k) if d == dv else k.new_empty((n, max_len, G, dv))
-    _check(_kv8_fn("ell_kv8_read")(*data, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), None, None, n, n, max_len, *sizes, *place,
-                                   _is_bf(dtype), _err_word(base.device), _stream()), "kv8_read")
+    _kv8_call("ell_kv8_read", "kv8_read", 1, *words, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), 0, 0, n, n, max_len, _is_bf(dtype),
+              _err_word(dev))
     return k, v
 
 
@@ -359,36 +348,34 @@ KV8_READ_ROWS, KV8_READ_BYTES = 512, 1 << 30
 KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 256, 444, 4232
 
 
-def _attention_read_back(q, cache, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):
-    T, n, dev = q.shape[0], cu_seqlens.numel() - 1, q.device
-    data, sizes, place = _kv8_parts(cache)
-    k, v = (torch.empty(n * max_len, sizes[0], w, dtype=q.dtype, device=dev) for w in sizes[1:])
+def _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):
+    T, n, G, dev = q.shape[0], cu_seqlens.numel() - 1, words[4], q.device
+    k, v = (torch.empty(n * max_len, G, w, dtype=q.dtype, device=dev) for w in words[5:7])
     rows = torch.empty(T, dtype=torch.int32, device=dev)
-    _check(_kv8_fn("ell_kv8_read")(*data, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(), rows.data_ptr(), n, T,
-                                   max_len, *sizes, *place, _is_bf(q.dtype), _err_word(dev), _stream()), "kv8_read")
+    _kv8_call("ell_kv8_read", "kv8_read", 1, *words, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(), rows.data_ptr(), n,
+              T, max_len, _is_bf(q.dtype), _err_word(dev))
     out = attention_rows(q, k, v, rows, length, max_len, scale, sink, alibi_slopes, window, None, cu_seqlens, max_q)
-    _check(_kv8_fn("ell_kv8_clear")(out.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(), n, T, out.shape[1] * out.shape[2], _stream()), "kv8_clear")
+    _check(lib().ell_kv8_clear(_p(out), _p(length), _p(cu_seqlens), c_int(n), c_int(T), c_int(out.shape[1] * out.shape[2]), _stream()), "kv8_clear")
     return out
 
 
 @_on_device
-def attention_kv8(q, cache, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):
-    (T, H, d), (data, sizes, place) = q.shape, _kv8_parts(cache)
-    G, _, dv = sizes
+def attention_kv8(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):
+    (T, H, d), G, dv = q.shape, words[4], words[6]
     window = window or 0
     n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, max_q)
     if max_q * (H // G) >= KV8_READ_ROWS and q.dtype is torch.bfloat16 and not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4) and \
             2 * n_seq * max_len * G * (d + dv) <= KV8_READ_BYTES:
-        return _attention_read_back(q, cache, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
+        return _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
     out = q.new_empty((T, H, dv))
-    # room for what shares cut (csrc/kv8.cu): a call has no more CTAs than are resident, or a CTA for each key head and 16 of its query heads
+    # room for what shares cut: a call has no more CTAs than are resident, or a CTA for each key head and 16 of its query heads
     need = max(KV8_CTAS, G * -(-(H // G) // 16)) * KV8_CTA_FLOATS if max_len > KV8_UNCUT else 0
     part = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
     sl = None if alibi_slopes is None else cu._slopes(alibi_slopes, H, q.device)
-    _check(_kv8_fn("ell_attn_kv8")(q.data_ptr(), *data, out.data_ptr(), None if part is None else part.data_ptr(), need, base.data_ptr(), length.data_ptr(),
-                                   None if sink is None else _f32(sink, "sink").data_ptr(), None if sl is None else sl.data_ptr(),
-                                   None if cu_seqlens is None else cu_seqlens.data_ptr(), T, n_seq, max_q, H, *sizes, _packed(q, "q"), max_len, window,
-                                   scale, *place, _is_bf(q.dtype), _err_word(q.device), _stream()), "attn_kv8", 2 if need else 1)
+    _kv8_call("ell_attn_kv8", "attn_kv8", 2 if need else 1, *words, q.data_ptr(), out.data_ptr(), 0 if part is None else part.data_ptr(), need, base.data_ptr(),
+              length.data_ptr(), 0 if sink is None else _f32(sink, "sink").data_ptr(), 0 if sl is None else sl.data_ptr(),
+              0 if cu_seqlens is None else cu_seqlens.data_ptr(), T, n_seq, max_q, H, _packed(q, "q"), max_len, window, _is_bf(q.dtype), _err_word(q.device),
+              scale)
     return out
 
 

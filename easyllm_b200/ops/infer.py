@@ -268,7 +268,8 @@ def kv8_empty(rows, heads, dim, vdim, block, device=None):
 
 
 def _kv8_check(cache, *ints):
-    """Raises where ``cache`` is not a ``KV8``, or an index vector not one; a serving step asks once a call, so it is put briefly."""
+    """What the kernels need to know of ``cache``: addresses, heads, head sizes, rows of a block and in all.  Raises where it is not a ``KV8``,
+    or an index vector not one."""
     k, v, ks, vs, d, dv = cache
     (R, G, wk), (Rv, Gv, wv), (B, Gs), dev = k.shape, v.shape, ks.shape, k.get_device()
     block = R // B if B else 0
@@ -281,6 +282,7 @@ def _kv8_check(cache, *ints):
     for t in ints:
         if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.get_device() != dev:
             raise ValueError("places and lengths of cache rows are contiguous int32 vectors on the cache's device")
+    return k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), G, d, dv, block, R
 
 
 def kv8_append(cache, k, v, meta):
@@ -290,24 +292,24 @@ def kv8_append(cache, k, v, meta):
     A block that has rows already keeps the larger scale; if that is the new one, its rows are rounded again."""
     no_grad_check(k, v)
     base, length, cu = meta["kv_base"], meta["kv_len"], meta["cu_seqlens"]
-    _kv8_check(cache, base, length, cu)
-    T, G = k.shape[0], cache.k.shape[1]
-    if k.shape != (T, G, cache.dim) or v.shape != (T, G, cache.vdim) or k.dtype != v.dtype or not k.get_device() == v.get_device() == base.get_device() or \
+    words = _kv8_check(cache, base, length, cu)
+    T, G = k.shape[0], words[4]
+    if k.shape != (T, G, words[5]) or v.shape != (T, G, words[6]) or k.dtype != v.dtype or not k.get_device() == v.get_device() == base.get_device() or \
             base.numel() != T or length.numel() != T:
         raise ValueError(f"kv8_append: k [T, {G}, {cache.dim}] and v [T, {G}, {cache.vdim}] of one dtype, a place and a length for each row")
     if _kern(k):
-        return _cu().kv8_append(k, v, cache, base, length, cu, meta["max_seqlen"])
+        return _cu().kv8_append(k, v, words, base, length, cu, meta["max_seqlen"])
     ref.kv8_append(cache, k, v, meta)
 
 
 def kv8_read(cache, kv_base, kv_len, max_len, dtype=torch.bfloat16):
     """The values of ``cache`` as keys ``[n, max_len, G, dim]`` and values ``[n, max_len, G, vdim]``: for each sequence the rows ``kv_base`` ..
     ``kv_base + kv_len`` (at most ``max_len``), then zeros.  Exact in bf16 and fp32."""
-    _kv8_check(cache, kv_base, kv_len)
+    words = _kv8_check(cache, kv_base, kv_len)
     if kv_base.shape != kv_len.shape or dtype not in (torch.bfloat16, torch.float32) or max_len < 0:
         raise ValueError("kv8_read: a place and a length for each sequence, into bf16 or fp32")
     if cache.k.is_cuda:
-        return _cu().kv8_read(kv_base, kv_len, cache, max_len, dtype)
+        return _cu().kv8_read(kv_base, kv_len, words, max_len, dtype)
     return ref.kv8_read(cache, kv_base, kv_len, max_len, dtype)
 
 
@@ -318,9 +320,9 @@ def attention_kv8(q, cache, kv_base, kv_len, max_len, scale, sink=None, alibi_sl
     border) are zero."""
     no_grad_check(q)
     ints = (kv_base, kv_len) if cu_seqlens is None else (kv_base, kv_len, cu_seqlens)
-    _kv8_check(cache, *ints)
+    words = _kv8_check(cache, *ints)
     T, H, d = q.shape
-    if d != cache.dim or H % cache.k.shape[1] or q.get_device() != kv_base.get_device() or kv_base.numel() != T or kv_len.numel() != T:
+    if d != words[5] or H % words[4] or q.get_device() != kv_base.get_device() or kv_base.numel() != T or kv_len.numel() != T:
         raise ValueError(f"attention_kv8: q [T, H, {cache.dim}] with a multiple of {cache.k.shape[1]} heads, a place and a length for each row")
     if window is not None and window < 1:
         raise ValueError(f"attention_kv8: a window of {window} rows")
@@ -330,7 +332,7 @@ def attention_kv8(q, cache, kv_base, kv_len, max_len, scale, sink=None, alibi_sl
     if cu_seqlens is not None and max_q is None:
         raise ValueError("attention_kv8: cu_seqlens comes with max_q, a bound of the sequences' rows")
     if _kern(q):
-        return _cu().attention_kv8(q, cache, kv_base, kv_len, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
+        return _cu().attention_kv8(q, words, kv_base, kv_len, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
     return ref.attention_kv8(q, cache, kv_base, kv_len, scale, sink, alibi_slopes, window, cu_seqlens)
 
 
