@@ -319,7 +319,7 @@ constexpr int kK8Threads = 128, kK8Keys = 64, kK8Stage = kK8Keys * 128;       //
 // kernels find their L1 cut down by).
 template <int NB>
 struct K8Ring {
-  static constexpr int kStages = NB == 1 ? 2 : 3, kCtas = NB == 1 ? 3 : 2, kBytes = 4 * kStages * kK8Stage;
+  static constexpr int kStages = 3, kCtas = 2, kBytes = 4 * kStages * kK8Stage;
   uint64_t full[4][kStages];
   int gave_up, free_stage[4];
   int piece[4];                   // of the current piece: first token, rows, where it begins, quanta behind its end
@@ -353,7 +353,8 @@ struct Kv8Attn {
 __host__ __device__ __forceinline__ int k8_groups(int H, int G) { return G * ((H / G + kK8Heads - 1) / kK8Heads); }
 
 // Work is counted in quanta of 256 keys, one unit of 64 for each warp of a CTA.  An item is a tile of `tt` tokens of a sequence (cu null: one
-// token) with the query heads of a key head, at most 16 of them.
+// token) with the query heads of a key head, at most 16 of them.  To begin an item costs a CTA as much as a quantum (queries, sums; 64
+// sequences of up to 8192 keys took 105.5 us without that in the shares, 103 with it).
 constexpr int kK8Quantum = 4 * kK8Keys;
 struct K8Tile {
   int r0, r1, base, len0, len1, low;              // low: where its keys begin, at a unit
@@ -378,14 +379,18 @@ struct K8Tile {
     low = max(0, len0 - a.window) & ~(kK8Keys - 1);
   }
   __device__ __forceinline__ int quanta() const { return r0 >= r1 ? 0 : max(1, (len1 - low + kK8Quantum - 1) / kK8Quantum); }
+  __device__ __forceinline__ int cost() const { return r0 >= r1 ? 0 : quanta() + 1; }
 };
-// What a CTA does at a time: quanta q0 .. q1 - 1 of a tile.
+// What a CTA does at a time: quanta q0 .. q1 - 1 of a tile.  From places in the tile's cost, of which the first is its beginning.
 struct K8Piece {
   K8Tile t;
-  int q0, q1, quanta;
-  __device__ __forceinline__ K8Piece(const Kv8Attn& a, int x, int q0_, int most) : t(a, x), q0(q0_) {
+  int q0, q1, quanta, behind;      // behind: cost of what is left of the tile
+  __device__ __forceinline__ K8Piece(const Kv8Attn& a, int x, int q0_, int most) : t(a, x) {
     quanta = t.quanta();
-    q1 = min(quanta, q0 + most);
+    const int end = min(t.cost(), q0_ + most);
+    behind = t.cost() - end;
+    q0 = max(0, q0_ - 1);
+    q1 = max(0, end - 1);
   }
   __device__ __forceinline__ int k0() const { return t.low + q0 * kK8Quantum; }
   __device__ __forceinline__ int k1() const { return min(t.low + q1 * kK8Quantum, t.len1); }
@@ -719,7 +724,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     // where the share begins: a lane counts the quanta of its tiles, and walks them if it is there; every warp for itself, without a barrier
     const int chunk = (n_x + 31) / 32, first = min(lane * chunk, n_x), last = min(first + chunk, n_x);
     int mine = 0;
-    for (int i = first; i < last; ++i) mine += K8Tile(a, i).quanta();
+    for (int i = first; i < last; ++i) mine += K8Tile(a, i).cost();
     int before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -738,7 +743,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     q0 = begin - before;
     if (here) {
       for (; x < last - 1; ++x) {
-        const int q = K8Tile(a, x).quanta();
+        const int q = K8Tile(a, x).cost();
         if (q0 < q) break;
         q0 -= q;
       }
@@ -779,12 +784,12 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   bool failed = false, fresh = true;
   while (true) {
     const K8Piece p(a, x, q0, left);
-    if (p.quanta == 0) return;                         // an item without rows (the shares have none)
+    if (p.q1 == p.q0) return;                          // an item without rows (the shares have none), or a share that ends where an item begins
     if (threadIdx.x == 0) {
       ring.piece[0] = p.t.r0;
       ring.piece[1] = (p.t.r1 - p.t.r0) * nh;
       ring.piece[2] = p.q0;
-      ring.piece[3] = p.quanta - p.q1;
+      ring.piece[3] = p.behind;
     }
     const int mine = p.units(warp), k0 = p.k0() + warp * kK8Keys, k1 = p.k1(), rows = (p.t.r1 - p.t.r0) * nh;
     if (fresh) {
@@ -792,7 +797,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       s_left = 2 * mine;
       fresh = false;
     }
-    left -= p.q1 - p.q0;
+    left -= p.t.cost() - p.behind - q0;
     send(kStages);
     // queries, scales and the next piece: what they need comes from memory together
     K8Query<T> query[NB];
@@ -1085,6 +1090,7 @@ struct Kv8AttnCall {
   int* err;
   double scale;
 };
+static_assert(sizeof(Kv8Args) == 9 * 8 && sizeof(Kv8AppendCall) == 21 * 8 && sizeof(Kv8ReadCall) == 20 * 8 && sizeof(Kv8AttnCall) == 28 * 8, "");
 static bool k8_cache(const Kv8Args& a, Kv8Cache& c) {
   const bool ok = a.G > 0 && a.G <= 65535 && a.d > 0 && a.dv > 0 && a.d <= kK8Dim && a.dv <= kK8Dim && a.block > 0 && a.block <= kK8MaxBlock &&
                   !(a.block & (a.block - 1)) && a.rows % a.block == 0 && a.rows <= 0x7fffffff;
@@ -1143,7 +1149,7 @@ ELL_API int ell_kv8_clear(void* out, const int* len, const int* cu, int n_seq, i
 }
 
 // q rows of ldq elements.  max_len bounds len[].  part (16-byte aligned): `part_floats` of scratch where max_len is above 256, enough for
-// max(444, key heads x groups of 16 query heads) x 4232.  window: keys a row sees (<= 0: all).  cu [n_seq + 1] (or null): rows
+// max(296, key heads x groups of 16 query heads) x 4232.  window: keys a row sees (<= 0: all).  cu [n_seq + 1] (or null): rows
 // cu[i] .. cu[i + 1] - 1 are consecutive tokens of one sequence, with one base and lengths that grow by one; max_q bounds their number.
 ELL_API int ell_attn_kv8(const Kv8AttnCall* call, cudaStream_t stream) {
   const Kv8AttnCall& x = *call;

@@ -345,7 +345,7 @@ def kv8_read(base, length, words, max_len, dtype):
 # Continued prompts: with this many rows (tokens times query heads of a key head) of a sequence, the cache's rows are written out in bf16 once
 # and the tcgen05 kernel attends to those; that takes memory for them.
 KV8_READ_ROWS, KV8_READ_BYTES = 512, 1 << 30
-KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 256, 444, 4232
+KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 256, 296, 4232
 
 
 def _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):

@@ -273,6 +273,9 @@ def check_attention(dev, dtype, H, G, d, dv, block, total, new, sink=False, alib
         for j in range(c):
             end = t - c + j + 1
             low = max(0, end - window) if window else 0
+            if T > 100 and r % 7 and j not in (0, c - 1):         # of long prompts some rows
+                r += 1
+                continue
             want, err = plain_attention(q[r], *(p.values(s * capacity + low, end - low) for p in plain), d ** -0.5, sk, sl)
             near(got[r], want, err)
             r += 1
@@ -553,3 +556,155 @@ def test_the_cache_is_asked_for_in_the_config():
     from megozen_models import CONFIGS
     with pytest.raises(ValueError):
         arch_from_hf_config(dict(CONFIGS["odd"], kv_cache_block=16))
+
+
+# ---- long continued prompts ---------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("device", ["cuda"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,G,d,dv,new,kind", [(8, 2, 128, 128, [150, 1, 300], None), (8, 1, 64, 32, [70, 131], "sink"), (4, 4, 128, 128, [1, 530], "alibi"),
+                                               (12, 2, 48, 128, [90, 1, 1, 200], "window"), (16, 2, 72, 128, [100, 20], None)])
+def test_attention_of_long_continued_prompts(device, dtype, H, G, d, dv, new, kind):
+    """Enough rows for the path through rows read back (bf16), and the same in fp32."""
+    dev = _device(device)
+    check_attention(dev, dtype, H, G, d, dv, 16, [601 + 77 * i for i in range(len(new))], new, sink=kind == "sink", alibi=kind == "alibi",
+                    window=150 if kind == "window" else None)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_long_prompts_beside_rows_that_see_nothing(device, dtype):
+    """A sequence without rows, one whose rows have length 0, rows behind the last border, a marked block."""
+    dev = _device(device)
+    H, G, d, n, cap = 8, 2, 64, 200, 512
+    cache, plain = filled(3 * cap, G, d, d, 16, dev)
+    cache.v_scale[(cap + 48) // 16, 1] = math.nan                 # values 48 .. 64 of the second sequence, head 1
+    q = rand(2 * n + 9, H, d, seed=1).to(dtype).to(dev)
+    base = ints([0] * n + [cap] * n + [3, -1, 777, 1 << 30, 0, 0, 0, 0, 0], dev)
+    length = ints(list(range(201, 201 + n)) + list(range(1, n + 1)) + [0, 0, 0, 99, 5, 6, 7, 8, 9], dev)
+    cu = ints([0, n, n, 2 * n, 2 * n + 3], dev)
+    got = iops.attention_kv8(q, cache, base, length, 401, 0.125, cu_seqlens=cu, max_q=n)
+    assert not bool(got[2 * n:].any())
+    nan = got.isnan().all(-1).cpu()
+    want_nan = torch.zeros(2 * n + 9, H, dtype=torch.bool)
+    want_nan[n + 48:2 * n, 4:] = True
+    assert torch.equal(nan, want_nan) and torch.equal(got.isnan().any(-1).cpu(), want_nan)
+    for r in (0, 1, 77, n - 1, n, n + 1, n + 47):
+        seq, end = r // n, 201 + r if r < n else r - n + 1
+        near(got[r], *plain_attention(q[r], *(p.values(seq * cap, end) for p in plain), 0.125))
+
+
+# ---- streams, graphs, devices, places past 32 bits ------------------------------------------------------------
+def _calls(dev, seed, dtype=BF16):
+    """A step of three sequences as closures over its own buffers: append, attend, read."""
+    H, G, d, cap = 8, 2, 128, 512
+    cache, _ = filled(3 * cap, G, d, d, 16, dev, seed=seed)
+    meta = step([1, 1, 1], [300, 17, 511], [2, 0, 1], cap, dev)
+    k, v, q = (rand(3, n, d, seed=seed + i).to(dtype).to(dev) for i, n in enumerate((G, G, H)))
+    base, length = meta["kv_base"], meta["kv_len"]
+
+    def run():
+        iops.kv8_append(cache, k, v, meta)
+        o = iops.attention_kv8(q, cache, base, length, cap, d ** -0.5)
+        return (o,) + iops.kv8_read(cache, base, length, cap)
+    return run, (k, v, q), cache
+
+
+@pytest.mark.gpu
+def test_two_captured_steps_replay_beside_each_other():
+    """Two graphs of steps that share nothing but the library, replayed on two streams at once with new inputs: the bits of eager steps."""
+    dev = _device("cuda")
+    runs = [_calls(dev, 1), _calls(dev, 100)]
+    for run, _, _ in runs:
+        run()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for run, _, _ in runs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in runs]
+    for i in range(5):
+        for j, (_, inputs, _) in enumerate(runs):
+            for t in inputs:
+                t.copy_(rand(*t.shape, seed=7 * i + j).to(t.dtype))
+        torch.cuda.synchronize()
+        kept = [tuple(t.clone() for t in cache[:4]) for _, _, cache in runs]
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                for _ in range(3):
+                    g.replay()
+        torch.cuda.synchronize()
+        got = [tuple(t.clone() for t in o) for o in outs]
+        for (run, _, cache), before, g in zip(runs, kept, got):
+            for t, b in zip(cache[:4], before):
+                t.copy_(b)
+            for a, b in zip(g, run()):
+                assert torch.equal(a, b)
+    from easyllm_b200.ops import cuda
+    cuda.check_err_flag()
+
+
+@pytest.mark.gpu
+def test_on_another_stream_and_again_on_the_same_inputs():
+    dev = _device("cuda")
+    run, _, _ = _calls(dev, 5)
+    want = run()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = [run() for _ in range(20)]
+    s.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+@pytest.mark.gpu
+def test_rows_past_two_gigabytes():
+    """A cache of more than 2^31 bytes: the places of its last rows."""
+    dev = _device("cuda")
+    G, d, B, rows = 16, 128, 16, (1 << 20) + 4096
+    cache = iops.kv8_empty(rows, G, d, d, B, dev)
+    assert cache.k.numel() > 1 << 31
+    n, base = 301, rows - 512
+    k, v, q = (rand(n, h, d, seed=h + i).to(BF16).to(dev) for i, h in enumerate((G, G, 2 * G)))
+    meta = {"kv_base": ints([base] * n, dev), "kv_len": ints(list(range(1, n + 1)), dev), "cu_seqlens": ints([0, n], dev), "max_seqlen": n}
+    iops.kv8_append(cache, k, v, meta)
+    plain = [Plain(512, G, d, B) for _ in range(2)]
+    for p, x in zip(plain, (k, v)):
+        p.append(0, 0, x)
+    for x, p in zip(iops.kv8_read(cache, ints([base], dev), ints([n], dev), n, F32), plain):
+        assert torch.equal(x[0].double().cpu(), p.values(0, n))
+    near(iops.attention_kv8(q[-1:], cache, ints([base], dev), ints([n], dev), n, 0.1)[0], *plain_attention(q[-1], *(p.values(0, n) for p in plain), 0.1))
+    got = iops.attention_kv8(q, cache, meta["kv_base"], meta["kv_len"], n, 0.1, cu_seqlens=meta["cu_seqlens"], max_q=n)
+    near(got[-1], *plain_attention(q[-1], *(p.values(0, n) for p in plain), 0.1))
+
+
+@pytest.mark.gpu
+def test_a_decoding_model_replays_its_graph():
+    """Generation with and without the captured decode step gives the same tokens, in bf16, and so does a state that is used again."""
+    dev = _device("cuda")
+    m = _model("llama", dev, BF16, kv_cache_block=16, hidden_size=512, num_attention_heads=4, num_key_value_heads=2)
+    ids = torch.randint(0, 97, (3, 40), generator=torch.Generator().manual_seed(3)).to(dev)
+    a = m.generate(ids, max_new_tokens=24)
+    b = m.generate(ids, max_new_tokens=24, cuda_graph=False)
+    assert a.shape == (3, 64) and torch.equal(a, b) and torch.equal(a, m.generate(ids, max_new_tokens=24))
+
+
+@pytest.mark.gpu
+def test_arguments_are_looked_over_on_a_gpu_too():
+    dev = _device("cuda")
+    cache = iops.kv8_empty(64, 2, 32, 16, 16, dev)
+    one = ints([0], dev)
+    with pytest.raises(ValueError):                               # an index on the host
+        iops.attention_kv8(torch.zeros(1, 4, 32, device=dev), cache, ints([0]), one, 4, 1.0)
+    with pytest.raises(ValueError):                               # queries on the host
+        iops.attention_kv8(torch.zeros(1, 4, 32), cache, one, one, 4, 1.0)
+    with pytest.raises(ValueError):                               # heads that are not packed
+        iops.attention_kv8(torch.zeros(2, 32, 4, device=dev).transpose(1, 2), cache, ints([0, 0], dev), ints([1, 1], dev), 4, 1.0)
+    with pytest.raises(ValueError):
+        iops.attention_kv8(torch.zeros(1, 4, 32, device=dev), cache, one, one, 4, 1.0, sink=torch.zeros(4))
+    with pytest.raises(ValueError):
+        iops.kv8_append(cache, torch.zeros(1, 2, 32), torch.zeros(1, 2, 16), step([1], [0], [0], 64, dev))
