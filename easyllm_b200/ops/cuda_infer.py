@@ -342,9 +342,11 @@ def kv8_read(base, length, words, max_len, dtype):
     return k, v
 
 
-# Continued prompts: with this many rows (tokens times query heads of a key head) of a sequence, the cache's rows are written out in bf16 once
-# and the tcgen05 kernel attends to those; that takes memory for them.
-KV8_READ_ROWS, KV8_READ_BYTES = 512, 1 << 30
+# Continued prompts with many rows (tokens times query heads of a key head): the cache's rows are written out in bf16 once and the tcgen05 kernel
+# attends to those, while that takes no more memory than this.  Us of the integer products on the cache | of rows read back (sequences, keys,
+# query and key heads, rows): 1 of 4096, 32/8, 128 rows 29 | 31, 256 43 | 37, 512 69 | 51, 2048 219 | 108; 1 of 4096, 32/32, 128 70 | 74, 256 123 |
+# 100; 1 of 30000, 64/8, 128 108 | 91, 256 195 | 126; 8 of 2000, 32/8, 256 58 | 67, 512 102 | 107, 1024 192 | 120; 2 of 400, 32/8, 256 21 | 27, 512 29 | 27.
+KV8_READ_ROWS, KV8_READ_LONG, KV8_READ_BYTES = 512, (256, 4096), 1 << 30
 KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 256, 296, 4232
 
 
@@ -364,7 +366,8 @@ def attention_kv8(q, words, base, length, max_len, scale, sink, alibi_slopes, wi
     (T, H, d), G, dv = q.shape, words[4], words[6]
     window = window or 0
     n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, max_q)
-    if max_q * (H // G) >= KV8_READ_ROWS and q.dtype is torch.bfloat16 and not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4) and \
+    rows = max_q * (H // G)
+    if (rows >= KV8_READ_ROWS or (rows >= KV8_READ_LONG[0] and max_len >= KV8_READ_LONG[1])) and q.dtype is torch.bfloat16 and not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4) and \
             2 * n_seq * max_len * G * (d + dv) <= KV8_READ_BYTES:
         return _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
     out = q.new_empty((T, H, dv))

@@ -6,7 +6,7 @@ Cases: gemm_nt, gemm_nt_n4096, gemm_dgrad, gemm_wgrad, gemm_ag, gemm_rs, gemm_ar
 the prefix gemm_pair_ (CTA-pair kernel) plus gemm_pair_agk (gather of the reduction rows into the weight-gradient
 GEMM) and gemm_pair_ce (LM head with the cross-entropy epilogue), flash_fwd, flash_bwd, rmsnorm_fwd, rmsnorm_bwd,
 swiglu, rope, adam, ce, attn_latent (decoding, 64 sequences of 4096 tokens, 32 heads over a latent of 512 + 64),
-attn_decode (64 sequences of 2100 keys), attn_continue (151 tokens each of two sequences over 3000 keys),
+attn_decode (64 sequences of 2100 keys), attn_kv8 (the same over an 8-bit cache), attn_continue (151 tokens each of two sequences over 3000 keys),
 flash_latent (one prompt of 4096 tokens, keys of 128 + 64, a window of 1024).
 Inputs are larger than L2 (126 MB) where the op is memory-bound but hold well under a few GB,
 so a full-section profiler capture of 1-3 launches ends by itself in a minute or two.
@@ -123,6 +123,14 @@ def main():
         ln = torch.arange(length - new + 1, length + 1, **i32).repeat(n)
         cus = torch.arange(0, n * new + 1, new, **i32) if new > 1 else None
         fn = lambda: ci.attention_rows(q, k, v, base, ln, length, 128 ** -0.5, cu_seqlens=cus, max_q=new)   # noqa: E731
+    elif c == "attn_kv8":
+        from . import infer as iops
+        i32 = dict(dtype=torch.int32, device="cuda")
+        cache = iops.kv8_empty(64 * 2304, 8, 128, 128, 16, "cuda")
+        cache.k.random_(-127, 128), cache.v.random_(-127, 128), cache.k_scale.fill_(2.0 ** -5), cache.v_scale.fill_(2.0 ** -5)
+        q = torch.randn(64, 32, 128, **bf)
+        base, ln = torch.arange(0, 64 * 2304, 2304, **i32), torch.full((64,), 2100, **i32)
+        fn = lambda: iops.attention_kv8(q, cache, base, ln, 2100, 128 ** -0.5)          # noqa: E731
     elif c == "flash_latent":
         from . import cuda_infer as ci
         z = torch.randn(4096, 32 * 192 + 576, **bf); kv = torch.randn(4096, 32 * 256, **bf)
