@@ -133,10 +133,9 @@ __global__ void __launch_bounds__(256, 4) kv8_append_kernel(const Kv8Cache c, co
   if (p0 < 0) return;                                             // padding
   const int b = (p0 >> c.shift) + j, start = b << c.shift, first = max(p0, start), last = min(p0 + count, start + (1 << c.shift));
   if (first >= last) return;
-  if (!k8_inside(c, base, p0 + count)) {
-    if (lane == 0) atomicCAS(err, 0, kK8Place);
-    return;
-  }
+  const bool inside = k8_inside(c, base, p0 + count);
+  if (lane == 0 && (!inside || (j == blocks - 1 && last < p0 + count))) atomicCAS(err, 0, kK8Place);      // more rows than was said are left out
+  if (!inside) return;
   const int width = which ? c.dv : c.d, row = k8_row(width), step = c.G * row, rows = last - first;
   const size_t ld = which ? ldv : ldk;
   const T* src = (which ? v : k) + (size_t)(r0 + first - p0) * ld + (size_t)g * width;
@@ -243,7 +242,7 @@ __device__ __forceinline__ void k8_store_values(T* o, const uint32_t* w, float s
 }
 // ko [n, max_len, G, d], vo [n, max_len, G, dv].  cu null: rows base[i] .. base[i] + len[i] - 1 of the cache, then zeros.  Otherwise sequence i has
 // the query rows cu[i] .. cu[i + 1] - 1 with base and len of their own: its rows are those that its last one sees, nothing is written behind them,
-// and row_base[r] becomes the place of a query row's keys in ko.  A thread keeps its place in a row, V elements, and takes positions, eight of which are
+// row_base[r] becomes the place of a query row's keys in ko, row_base[rows + r] its length, max_len at most.  A thread keeps its place in a row, V elements, and takes positions, eight of which are
 // under way together.  Bound by memory: 8 prefixes of up to 4096 rows, 8 heads of 128 (37 MB in, 134 MB out, zeros among them) 31 us, 5.5 TB/s.  With
 // a division for every eight values it took 48 us, with conversions of the integers 39, with 16 values a thread, whose stores leave
 // every other 16 bytes to the next one, 134.
@@ -259,11 +258,14 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Cache c, T* __re
     r1 = min(cu[i + 1], rows);
     if (r0 < 0 || r0 >= r1) return;
     if (blockIdx.x == 0)
-      for (int r = r0 + threadIdx.x; r < r1; r += 256) row_base[r] = i * max_len;
+      for (int r = r0 + threadIdx.x; r < r1; r += 256) {
+        row_base[r] = i * max_len;
+        row_base[rows + r] = min(len[r], max_len);
+      }
   }
   const int first = base[r0], n = min(len[r1 - 1], max_len);
   const bool ok = n <= 0 || k8_inside(c, first, n);
-  if (!ok && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(err, 0, kK8Place);
+  if ((!ok || (cu != nullptr && len[r1 - 1] > max_len)) && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(err, 0, kK8Place);
   const int p0 = blockIdx.x * chunk, p1 = min(p0 + chunk, cu != nullptr && ok ? n : max_len);
   const int beside = max(1, 256 / per);                          // positions that the threads take side by side
   for (int y = threadIdx.x; y < beside * per; y += 256) {
@@ -383,6 +385,7 @@ struct K8Tile {
     len0 = len1 = low = base = 0;
     if (r0 < 0) r1 = r0;
     if (r0 >= r1) return;
+    if (a.cu != nullptr && x % a.tiles == a.tiles - 1 && r1 < min(a.cu[x / a.tiles + 1], a.n)) atomicCAS(a.err, 0, kK8Place);      // more tokens than was said
     len0 = a.len[r0];
     len1 = a.len[r1 - 1];
     base = a.base[r0];
@@ -751,7 +754,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     const int begin = k8_share(share, all, shares);
     left = share < shares ? k8_share(share + 1, all, shares) - begin : 0;
     if (threadIdx.x == 0) reinterpret_cast<K8Cut*>(a.part + (size_t)gridDim.x * 2 * R * LD)[blockIdx.x].more = 0;
-    if (left == 0) return;
+    if (left <= 0) return;
     const bool here = begin >= before && begin < before + mine;
     x = first;
     q0 = begin - before;
@@ -763,6 +766,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       }
     }
     const int who = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    if (who < 0) return;
     x = __shfl_sync(0xffffffffu, x, who);
     q0 = __shfl_sync(0xffffffffu, q0, who);
   }
@@ -1045,6 +1049,7 @@ static K8Plan k8_plan(int n, int n_seq, int max_q, int H, int G, int max_len, in
   if (window > 0) max_len = std::min<long long>(max_len, (long long)window + p.tt + kK8Keys);      // rows see windows that start apart
   const long long x = n_seq > 0 ? (long long)n_seq * p.tiles : n, hs = k8_groups(H, G), quanta = std::max(1, (max_len + kK8Quantum - 1) / kK8Quantum),
                   resident = (long long)kNumSMs * (p.nb == 1 ? K8Ring<1>::kCtas : K8Ring<2>::kCtas);
+  if (x * hs > 0x7fffffff || x * (quanta + 2) > 0x7fffffff) return p;      // not to be counted in 32 bits: ctas 0
   p.cut = quanta > 1;
   p.ctas = (int)std::min<long long>((p.cut ? std::min(std::max(1ll, resident / hs), x * quanta) : x) * hs, 0x7fffffff);
   return p;
@@ -1134,7 +1139,7 @@ ELL_API int ell_kv8_append(const Kv8AppendCall* call, cudaStream_t stream) {
   return launch_status();
 }
 
-// cu [n + 1] and row_base [rows_q] (or null, null): see kv8_read_kernel.
+// cu [n + 1] and row_base [2, rows_q] (or null, null): see kv8_read_kernel.
 ELL_API int ell_kv8_read(const Kv8ReadCall* call, cudaStream_t stream) {
   const Kv8ReadCall& x = *call;
   Kv8Cache c;

@@ -353,10 +353,10 @@ KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 256, 296, 4232
 def _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):
     T, n, G, dev = q.shape[0], cu_seqlens.numel() - 1, words[4], q.device
     k, v = (torch.empty(n * max_len, G, w, dtype=q.dtype, device=dev) for w in words[5:7])
-    rows = torch.empty(T, dtype=torch.int32, device=dev)
+    rows = torch.empty(2, T, dtype=torch.int32, device=dev)
     _kv8_call("ell_kv8_read", "kv8_read", 1, *words, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(), rows.data_ptr(), n,
               T, max_len, _is_bf(q.dtype), _err_word(dev))
-    out = attention_rows(q, k, v, rows, length, max_len, scale, sink, alibi_slopes, window, None, cu_seqlens, max_q)
+    out = attention_rows(q, k, v, rows[0], rows[1], max_len, scale, sink, alibi_slopes, window, None, cu_seqlens, max_q)
     _check(lib().ell_kv8_clear(_p(out), _p(length), _p(cu_seqlens), c_int(n), c_int(T), c_int(out.shape[1] * out.shape[2]), _stream()), "kv8_clear")
     return out
 

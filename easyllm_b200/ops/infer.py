@@ -288,14 +288,14 @@ def _kv8_check(cache, *ints):
 def kv8_append(cache, k, v, meta):
     """Quantise the step's keys k ``[T, G, dim]`` and values v ``[T, G, vdim]`` into their places of ``cache``: the rows between two borders
     of ``meta["cu_seqlens"]`` are the next tokens of one sequence, of which the first goes to row ``kv_base + kv_len - 1`` (a sequence starts
-    at a block; the sequences of a step are distinct).  Rows behind the last border, and sequences whose ``kv_len`` is 0, are left out.
+    at a block; the sequences of a step are distinct).  ``meta["max_seqlen"]`` bounds their numbers.  Rows behind the last border, and sequences whose ``kv_len`` is 0, are left out.
     A block that has rows already keeps the larger scale; if that is the new one, its rows are rounded again."""
     no_grad_check(k, v)
     base, length, cu = meta["kv_base"], meta["kv_len"], meta["cu_seqlens"]
     words = _kv8_check(cache, base, length, cu)
     T, G = k.shape[0], words[4]
     if k.shape != (T, G, words[5]) or v.shape != (T, G, words[6]) or k.dtype != v.dtype or not k.get_device() == v.get_device() == base.get_device() or \
-            base.numel() != T or length.numel() != T:
+            base.numel() != T or length.numel() != T or cu.numel() < 1:
         raise ValueError(f"kv8_append: k [T, {G}, {cache.dim}] and v [T, {G}, {cache.vdim}] of one dtype, a place and a length for each row")
     if _kern(k):
         return _cu().kv8_append(k, v, words, base, length, cu, meta["max_seqlen"])
@@ -329,8 +329,8 @@ def attention_kv8(q, cache, kv_base, kv_len, max_len, scale, sink=None, alibi_sl
     for t, name in ((sink, "sink"), (alibi_slopes, "alibi_slopes")):
         if t is not None and (t.numel() != H or t.get_device() != q.get_device()):
             raise ValueError(f"attention_kv8: {name} has one value for each of the {H} heads on their device")
-    if cu_seqlens is not None and max_q is None:
-        raise ValueError("attention_kv8: cu_seqlens comes with max_q, a bound of the sequences' rows")
+    if cu_seqlens is not None and (max_q is None or cu_seqlens.numel() < 1):
+        raise ValueError("attention_kv8: cu_seqlens has a border at least, and comes with max_q, a bound of the sequences' rows")
     if _kern(q):
         return _cu().attention_kv8(q, words, kv_base, kv_len, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
     return ref.attention_kv8(q, cache, kv_base, kv_len, scale, sink, alibi_slopes, window, cu_seqlens)

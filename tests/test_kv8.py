@@ -407,9 +407,11 @@ def test_refusals():
             iops.kv8_append(cache, k, v, dict(meta, **{name: meta[name].long()}))
     ok = dict(q=q, cache=cache, kv_base=one, kv_len=one, max_len=4, scale=1.0)
     for change in (dict(q=torch.zeros(1, 4, 16)), dict(q=torch.zeros(1, 3, 32)), dict(kv_len=ints([1, 2])), dict(kv_len=one.long()), dict(window=0),
-                   dict(sink=torch.zeros(3)), dict(alibi_slopes=torch.zeros(2)), dict(cu_seqlens=ints([0, 1]))):
+                   dict(sink=torch.zeros(3)), dict(alibi_slopes=torch.zeros(2)), dict(cu_seqlens=ints([0, 1])), dict(cu_seqlens=ints([]), max_q=1)):
         with pytest.raises(ValueError):
             iops.attention_kv8(**{**ok, **change})
+    with pytest.raises(ValueError):
+        iops.kv8_append(cache, k, v, dict(meta, cu_seqlens=ints([])))
     with pytest.raises(ValueError):
         iops.kv8_read(cache, one, one, 4, torch.float16)
     with pytest.raises(RuntimeError):
@@ -447,6 +449,28 @@ def test_places_outside_the_cache_are_reported(base, n):
         assert out is None or not bool(out.any())
     for x, p in zip(iops.kv8_read(cache, ints([0], dev), ints([64], dev), 64, F32), plain):
         assert torch.equal(x[0].double().cpu(), p.values(0, 64))
+
+
+@pytest.mark.gpu
+def test_bounds_that_are_exceeded_are_reported():
+    """More rows of a sequence, or longer ones, than the call was told: the error word is set, and nothing outside is touched."""
+    from easyllm_b200.ops import cuda
+    dev = _device("cuda")
+    cache, plain = filled(1024, 2, 32, 32, 16, dev)
+    k, v = rand(70, 2, 32, seed=1).to(dev), rand(70, 2, 32, seed=2).to(dev)
+    meta = step([70], [0], [0], 1024, dev)
+    iops.kv8_append(cache, k, v, dict(meta, max_seqlen=3))
+    with pytest.raises(cuda.KernelError, match="51"):
+        cuda.check_err_flag()
+    q = rand(300, 4, 32, seed=3).to(BF16).to(dev)
+    meta = step([300], [500], [0], 1024, dev)
+    cache, plain = filled(1024, 2, 32, 32, 16, dev)
+    for max_q, max_len in ((8, 800), (300, 600)):                 # the second through rows read back, whose kernels stop at an error
+        got = iops.attention_kv8(q, cache, meta["kv_base"], meta["kv_len"], max_len, 0.2, cu_seqlens=meta["cu_seqlens"], max_q=max_q)
+        with pytest.raises(cuda.KernelError, match="51"):
+            cuda.check_err_flag()
+        for r in range(8 if max_q == 8 else 0):
+            near(got[r], *plain_attention(q[r], *(p.values(0, 501 + r) for p in plain), 0.2))
 
 
 # ---- a run of them together -------------------------------------------------------------------------------
