@@ -1050,7 +1050,10 @@ static K8Plan k8_plan(int n, int n_seq, int max_q, int H, int G, int max_len, in
   const long long x = n_seq > 0 ? (long long)n_seq * p.tiles : n, hs = k8_groups(H, G), quanta = std::max(1, (max_len + kK8Quantum - 1) / kK8Quantum),
                   resident = (long long)kNumSMs * (p.nb == 1 ? K8Ring<1>::kCtas : K8Ring<2>::kCtas);
   if (x * hs > 0x7fffffff || x * (quanta + 2) > 0x7fffffff) return p;      // not to be counted in 32 bits: ctas 0
-  p.cut = quanta > 1;
+  // Up to 1024 keys an item a CTA: the join is a launch, 4 us.  Us cut | not (sequences of so many keys, 32 heads on 8): 1 of 500 9.4 | 7.2, of 1000
+  // 10.7 | 10.6, of 1500 11.0 | 13.9; 16 of 500 12.3 | 8.3, of 1000 13.2 | 12.7, of 1500 13.6 | 16.7; 64 of 700 22.4 | 19.1, of 1000 25.4 | 23.9, of
+  // 2000 36 | 40; 64 of 1000, 32 on 32, 72 | 70, of 2000 107 | 108.
+  p.cut = quanta > 4;
   p.ctas = (int)std::min<long long>((p.cut ? std::min(std::max(1ll, resident / hs), x * quanta) : x) * hs, 0x7fffffff);
   return p;
 }
@@ -1167,7 +1170,7 @@ ELL_API int ell_kv8_clear(void* out, const int* len, const int* cu, int n_seq, i
   return launch_status();
 }
 
-// q rows of ldq elements.  max_len bounds len[].  part (16-byte aligned): `part_floats` of scratch where max_len is above 256, enough for
+// q rows of ldq elements.  max_len bounds len[].  part (16-byte aligned): `part_floats` of scratch where max_len is above 1024, enough for
 // max(296, key heads x groups of 16 query heads) x 4232.  window: keys a row sees (<= 0: all).  cu [n_seq + 1] (or null): rows
 // cu[i] .. cu[i + 1] - 1 are consecutive tokens of one sequence, with one base and lengths that grow by one; max_q bounds their number.
 ELL_API int ell_attn_kv8(const Kv8AttnCall* call, cudaStream_t stream) {

@@ -347,7 +347,7 @@ def kv8_read(base, length, words, max_len, dtype):
 # query and key heads, rows): 1 of 4096, 32/8, 128 rows 29 | 31, 256 43 | 37, 512 69 | 51, 2048 219 | 108; 1 of 4096, 32/32, 128 70 | 74, 256 123 |
 # 100; 1 of 30000, 64/8, 128 108 | 91, 256 195 | 126; 8 of 2000, 32/8, 256 58 | 67, 512 102 | 107, 1024 192 | 120; 2 of 400, 32/8, 256 21 | 27, 512 29 | 27.
 KV8_READ_ROWS, KV8_READ_LONG, KV8_READ_BYTES = 512, (256, 4096), 1 << 30
-KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 256, 296, 4232
+KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 1024, 296, 4232
 
 
 def _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):

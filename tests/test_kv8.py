@@ -292,6 +292,16 @@ def test_attention_of_single_tokens(device, dtype, H, G, d, dv, block):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,G,d,dv,block", [(4, 4, 128, 128, 16), (8, 2, 128, 128, 1), (20, 1, 24, 128, 32), (34, 2, 128, 96, 128), (3, 3, 100, 7, 2)])
+def test_attention_over_lengths_that_shares_cut(device, dtype, H, G, d, dv, block):
+    """One sequence beyond 1024 keys among short ones: CTAs take shares of all keys, whose ends cut the sequences anywhere."""
+    dev = _device(device)
+    check_attention(dev, dtype, H, G, d, dv, block, [1, 1500, 256, 257, 31, 1100], [1] * 6, sink=True)
+    check_attention(dev, dtype, H, G, d, dv, block, [1300, 3, 5, 700], [3, 1, 5, 2], window=1200, alibi=True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("kind", ["sink", "alibi", "window", "all"])
 @pytest.mark.parametrize("new", [[1, 1, 1, 1], [3, 1, 2, 5], [40, 1, 77, 130]])
 def test_attention_with_sinks_slopes_and_windows(device, dtype, kind, new):
@@ -620,10 +630,10 @@ def test_long_prompts_beside_rows_that_see_nothing(device, dtype):
 
 # ---- streams, graphs, devices, places past 32 bits ------------------------------------------------------------
 def _calls(dev, seed, dtype=BF16):
-    """A step of three sequences as closures over its own buffers: append, attend, read."""
-    H, G, d, cap = 8, 2, 128, 512
+    """A step of three sequences as closures over its own buffers: append, attend (in shares, which are joined), read."""
+    H, G, d, cap = 8, 2, 128, 2048
     cache, _ = filled(3 * cap, G, d, d, 16, dev, seed=seed)
-    meta = step([1, 1, 1], [300, 17, 511], [2, 0, 1], cap, dev)
+    meta = step([1, 1, 1], [1300, 17, 2047], [2, 0, 1], cap, dev)
     k, v, q = (rand(3, n, d, seed=seed + i).to(dtype).to(dev) for i, n in enumerate((G, G, H)))
     base, length = meta["kv_base"], meta["kv_len"]
 
