@@ -28,8 +28,8 @@ struct Kv8Cache {
 __host__ __device__ __forceinline__ int k8_row(int d) { return (d + 15) / 16 * 16; }
 
 // Whether `n` rows from `base` on lie in the cache, from the start of a block.
-__device__ __forceinline__ bool k8_inside(const Kv8Cache& c, int base, int n) {
-  return base >= 0 && (base & ((1 << c.shift) - 1)) == 0 && (long long)base + n <= c.rows;
+__device__ __forceinline__ bool k8_inside(const Kv8Cache& c, int base, long long n) {
+  return base >= 0 && (base & ((1 << c.shift) - 1)) == 0 && base + n <= c.rows;
 }
 __device__ __forceinline__ float k8_scale_of(float amax) {       // amax finite, >= 0
   const int e = (int)((__float_as_uint(amax) + 0x1ffffu) >> 23) - 6;      // 127 = 2^6 (2 - 2^-6): carries above that mantissa
@@ -120,9 +120,9 @@ struct K8Elems<T, 1> {
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(256, 4) kv8_append_kernel(const Kv8Cache c, const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ base_,
-                                                            const int* __restrict__ len_, const int* __restrict__ cu, int n_seq, int n, int blocks,
-                                                            int ldk, int ldv, int* __restrict__ err) {
+__global__ void __launch_bounds__(256, 4)
+kv8_append_kernel(const Kv8Cache c, const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ base_, const int* __restrict__ len_,
+                  const int* __restrict__ cu, int n_seq, int n, int blocks, int ldk, int ldv, int* __restrict__ err) {
   chain_enter(k, v, base_, len_, cu, err);
   const unsigned item = blockIdx.x * 8u + (threadIdx.x >> 5), rest = item / c.G;
   const int lane = threadIdx.x & 31, g = (int)(item % c.G), which = (int)(rest & 1), j = (int)((rest >> 1) % blocks), s = (int)((rest >> 1) / blocks);
@@ -131,11 +131,13 @@ __global__ void __launch_bounds__(256, 4) kv8_append_kernel(const Kv8Cache c, co
   if (count <= 0 || r0 < 0) return;
   const int base = base_[r0], p0 = len_[r0] - 1;
   if (p0 < 0) return;                                             // padding
+  if (!k8_inside(c, base, (long long)p0 + count)) {
+    if (lane == 0) atomicCAS(err, 0, kK8Place);
+    return;
+  }
   const int b = (p0 >> c.shift) + j, start = b << c.shift, first = max(p0, start), last = min(p0 + count, start + (1 << c.shift));
   if (first >= last) return;
-  const bool inside = k8_inside(c, base, p0 + count);
-  if (lane == 0 && (!inside || (j == blocks - 1 && last < p0 + count))) atomicCAS(err, 0, kK8Place);      // more rows than was said are left out
-  if (!inside) return;
+  if (lane == 0 && j == blocks - 1 && last < p0 + count) atomicCAS(err, 0, kK8Place);      // more rows than was said: they are left out
   const int width = which ? c.dv : c.d, row = k8_row(width), step = c.G * row, rows = last - first;
   const size_t ld = which ? ldv : ldk;
   const T* src = (which ? v : k) + (size_t)(r0 + first - p0) * ld + (size_t)g * width;
@@ -222,7 +224,8 @@ __device__ __forceinline__ void k8_store_values(T* o, const uint32_t* w, float s
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t u = w[i / 2] ^ 0x80808080u;
-      f[i] = make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, i & 1 ? 0x7552 : 0x7550)), __uint_as_float(__byte_perm(u, 0x4b000000u, i & 1 ? 0x7553 : 0x7551)));
+      f[i] = make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, i & 1 ? 0x7552 : 0x7550)),
+                         __uint_as_float(__byte_perm(u, 0x4b000000u, i & 1 ? 0x7553 : 0x7551)));
       f[i] = sm100::fmul2(sm100::fadd2(f[i], make_float2(-8388736.f, -8388736.f)), make_float2(s, s));
     }
     if (kHalf) {
@@ -242,14 +245,14 @@ __device__ __forceinline__ void k8_store_values(T* o, const uint32_t* w, float s
 }
 // ko [n, max_len, G, d], vo [n, max_len, G, dv].  cu null: rows base[i] .. base[i] + len[i] - 1 of the cache, then zeros.  Otherwise sequence i has
 // the query rows cu[i] .. cu[i + 1] - 1 with base and len of their own: its rows are those that its last one sees, nothing is written behind them,
-// row_base[r] becomes the place of a query row's keys in ko, row_base[rows + r] its length, max_len at most.  A thread keeps its place in a row, V elements, and takes positions, eight of which are
-// under way together.  Bound by memory: 8 prefixes of up to 4096 rows, 8 heads of 128 (37 MB in, 134 MB out, zeros among them) 31 us, 5.5 TB/s.  With
-// a division for every eight values it took 48 us, with conversions of the integers 39, with 16 values a thread, whose stores leave
-// every other 16 bytes to the next one, 134.
+// row_base[r] becomes the place of a query row's keys in ko, row_base[rows + r] its length, max_len at most.  A thread keeps its place in a row, V
+// elements, and takes positions, eight of which are under way together.  Bound by memory: 8 prefixes of up to 4096 rows, 8 heads of 128 (37 MB
+// in, 134 MB out, zeros among them) 31 us, 5.5 TB/s.  With a division for every eight values it took 48 us, with conversions of the integers
+// 39, with 16 values a thread, whose stores leave every other 16 bytes to the next one, 134.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Cache c, T* __restrict__ ko, T* __restrict__ vo, const int* __restrict__ base,
-                                                       const int* __restrict__ len, const int* __restrict__ cu, int* __restrict__ row_base, int rows, int max_len,
-                                                       int chunk, int* __restrict__ err) {
+__global__ void __launch_bounds__(256)
+kv8_read_kernel(const Kv8Cache c, T* __restrict__ ko, T* __restrict__ vo, const int* __restrict__ base, const int* __restrict__ len,
+                const int* __restrict__ cu, int* __restrict__ row_base, int rows, int max_len, int chunk, int* __restrict__ err) {
   chain_enter(ko, vo, base, len, cu, row_base, err);
   const int i = blockIdx.y, pk = c.d / V, pv = c.dv / V, per = c.G * (pk + pv);
   int r0 = i, r1 = i + 1;
@@ -271,7 +274,8 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Cache c, T* __re
   for (int y = threadIdx.x; y < beside * per; y += 256) {
     const int z0 = y % per, at_p = y / per;
     const bool is_v = z0 >= c.G * pk;
-    const int z = is_v ? z0 - c.G * pk : z0, pieces = is_v ? pv : pk, width = is_v ? c.dv : c.d, g = z / pieces, at = z % pieces * V, row = k8_row(width);
+    const int z = is_v ? z0 - c.G * pk : z0, pieces = is_v ? pv : pk, width = is_v ? c.dv : c.d, row = k8_row(width);
+    const int g = z / pieces, at = z % pieces * V;
     const int step = c.G * row, out_step = c.G * width, mine = ok ? min(n, p1) : 0;
     const int8_t* q = (is_v ? c.v : c.k) + ((size_t)first * c.G + g) * row + at;
     const float* scale = (is_v ? c.vs : c.ks) + (size_t)(first >> c.shift) * c.G + g;
@@ -305,7 +309,8 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Cache c, T* __re
 }
 
 // Rows that see nothing, and those behind the last sequence, of out [n, width]: zero.
-__global__ void __launch_bounds__(256) kv8_clear_kernel(__nv_bfloat16* __restrict__ out, const int* __restrict__ len, const int* __restrict__ cu, int n_seq, int n, int width) {
+__global__ void __launch_bounds__(256)
+kv8_clear_kernel(__nv_bfloat16* __restrict__ out, const int* __restrict__ len, const int* __restrict__ cu, int n_seq, int n, int width) {
   chain_enter(out, len, cu);
   const int end = cu[n_seq];
   for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < n; t += gridDim.x * 8)
@@ -325,11 +330,11 @@ __global__ void __launch_bounds__(256) kv8_clear_kernel(__nv_bfloat16* __restric
 //           need no exchange, and four keys' bytes of a column come together by byte permutations
 //   rings   rows of 128 bytes with TMA's 128-byte swizzle: neither access meets a bank conflict
 // Bound by memory where sequences are long, by what begins and ends a call (3 us until the first copy, 5 for the join) where they are short.
-// Bytes of the cache a second, and us beside those of attention over the same cache in 16 bits: 64 sequences of up to 8192 keys, 32 heads on 8,
-// 5.6 TB/s, 99 (216); 24 of up to 4096, 32 on 32, 5.4, 78 (149); one of 131071, 64 on 8, 4.7, 58 (92); 6 of up to 1900 with 5 tokens each, 40 on 40, 2.5,
-// 27 (52); one of 203 keys 6.3 us (8.2).  Steps, us of the first two: a warp a row on the fp32 units 8398 and 4193; integer products with 32 keys
-// a step, a CTA an item 153 and 103; equal shares, 64 keys a step 119 and 100; found and joined with fewer barriers 110 and 91; two CTAs an SM with three
-// stages in place of three with two 105 and 86; items' beginnings counted 103 and 85.
+// Bytes of the cache a second, and us beside those of attention over the same cache in 16 bits: 64 sequences of up to 8192 keys, 32 heads
+// on 8, 5.6 TB/s, 99 (216); 24 of up to 4096, 32 on 32, 5.4, 78 (149); one of 131071, 64 on 8, 4.7, 58 (92); 6 of up to 1900 with 5 tokens
+// each, 40 on 40, 2.5, 27 (52); one of 203 keys 6.3 us (8.2).  Steps, us of the first two: a warp a row on the fp32 units 8398 and 4193;
+// integer products with 32 keys a step, a CTA an item 153 and 103; equal shares, 64 keys a step 119 and 100; found and joined with fewer
+// barriers 110 and 91; two CTAs an SM with three stages in place of three with two 105 and 86; items' beginnings counted 103 and 85.
 constexpr int kK8Threads = 128, kK8Keys = 64, kK8Stage = kK8Keys * 128;       // a stage: keys, or values
 // Stages of a warp and CTAs an SM, which are to fit a split of 196 KB with the system's 1 KB each (112 bytes more take 228 KB, which later
 // kernels find their L1 cut down by).
@@ -385,14 +390,17 @@ struct K8Tile {
     len0 = len1 = low = base = 0;
     if (r0 < 0) r1 = r0;
     if (r0 >= r1) return;
-    if (a.cu != nullptr && x % a.tiles == a.tiles - 1 && r1 < min(a.cu[x / a.tiles + 1], a.n)) atomicCAS(a.err, 0, kK8Place);      // more tokens than was said
+    if (a.cu != nullptr && x % a.tiles == a.tiles - 1 && r1 < min(a.cu[x / a.tiles + 1], a.n))
+      atomicCAS(a.err, 0, kK8Place);                   // more tokens than was said
     len0 = a.len[r0];
     len1 = a.len[r1 - 1];
     base = a.base[r0];
     if (len1 > 0 && !k8_inside(a.c, base, len1)) {
       atomicCAS(a.err, 0, kK8Place);
-      len0 = len1 = 0;
+      len1 = 0;
     }
+    len1 = max(len1, 0);
+    len0 = min(max(len0, 0), len1);
     low = max(0, len0 - a.window) & ~(kK8Keys - 1);
   }
   __device__ __forceinline__ int quanta() const { return r0 >= r1 ? 0 : max(1, (len1 - low + kK8Quantum - 1) / kK8Quantum); }
@@ -421,7 +429,8 @@ __device__ __forceinline__ int k8_next(const Kv8Attn& a, int n_x, int x) {
 }
 // Where share i of n begins among `all` quanta.
 __device__ __forceinline__ int k8_share(int i, int all, int n) {
-  return all < (1 << 20) ? (int)((unsigned)i * (unsigned)all / (unsigned)n) : (int)((long long)i * all / n);      // i is below 2^12 then, as the CTAs are
+  // shares are below 2^12, as CTAs that are resident are
+  return all < (1 << 20) ? (int)((unsigned)i * (unsigned)all / (unsigned)n) : (int)((long long)i * all / n);
 }
 // What the joining kernel needs to know of an item that begins in a CTA's share and is cut by its end.
 struct K8Cut {
@@ -448,15 +457,15 @@ constexpr uint32_t kMagic = 0x4b400000;
 // The left operand signed (queries) or not (weights).  `first`: a sum that starts here, from `zero`.
 template <bool SIGNED>
 __device__ __forceinline__ void mma_i8(int (&c)[4], bool first, const uint32_t (&zero)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-#define ELL_MMA(TYPE)                                                                                                                              \
-  if (first)                                                                                                                                       \
-    asm("mma.sync.aligned.m16n8k32.row.col.s32." TYPE ".s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"       \
-                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])                                                                                  \
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(zero[0]), "r"(zero[1]), "r"(zero[2]), "r"(zero[3]));                                                             \
-  else                                                                                                                                             \
-    asm("mma.sync.aligned.m16n8k32.row.col.s32." TYPE ".s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"           \
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])                                                                                  \
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+#define ELL_MMA(TYPE)                                                                                                                  \
+  if (first)                                                                                                                           \
+    asm("mma.sync.aligned.m16n8k32.row.col.s32." TYPE ".s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"    \
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])                                                                               \
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(zero[0]), "r"(zero[1]), "r"(zero[2]), "r"(zero[3]));       \
+  else                                                                                                                                 \
+    asm("mma.sync.aligned.m16n8k32.row.col.s32." TYPE ".s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"        \
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])                                                                               \
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   if (SIGNED) {
     ELL_MMA("s8")
   } else {
@@ -471,7 +480,9 @@ __device__ __forceinline__ uint32_t k8_kept(uint32_t x) {
   asm volatile("shfl.sync.idx.b32 %0, %1, 0, 31, 0xffffffff;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ float2 k8_sum(int x, int y) { return sm100::fadd2(make_float2(__int_as_float(x), __int_as_float(y)), make_float2(-kMagicF, -kMagicF)); }
+__device__ __forceinline__ float2 k8_sum(int x, int y) {
+  return sm100::fadd2(make_float2(__int_as_float(x), __int_as_float(y)), make_float2(-kMagicF, -kMagicF));
+}
 // high 2^16 + middle 2^8 + low of two sums
 __device__ __forceinline__ float2 k8_join(int l0, int l1, int m0, int m1, int h0, int h1) {
   const float2 b = make_float2(256.f, 256.f);
@@ -486,8 +497,8 @@ __device__ __forceinline__ void transpose_bytes(uint32_t a, uint32_t b, uint32_t
   y[3] = __byte_perm(ab1, cd1, 0x7632);
 }
 
-// The 32 elements 32 c .. 32 c + 31 of a query row, as they come, with what else a row of queries needs from memory: all of it is asked for before any
-// of it is looked at.
+// The 32 elements 32 c .. 32 c + 31 of a query row, as they come, with what else a row of queries needs from memory: all of it is asked for
+// before any of it is looked at.
 template <typename T>
 struct K8Query {
   static constexpr int kWords = 8 * sizeof(T);         // of 32 elements
@@ -573,8 +584,8 @@ struct K8Weights {
   uint32_t p[2][4], high[2][2];   // bytes, of 32 keys each: low and middle as an operand, high
   float before, now;
 };
-__device__ __forceinline__ void k8_softmax(const Kv8Attn& a, K8Rows& r, float (&s)[16], const float (&ks)[16], const float (&vs)[16], int key0, int c, bool mask,
-                                           K8Weights& w) {
+__device__ __forceinline__ void k8_softmax(const Kv8Attn& a, K8Rows& r, float (&s)[16], const float (&ks)[16], const float (&vs)[16], int key0,
+                                           int c, bool mask, K8Weights& w) {
 #pragma unroll
   for (int i = 0; i < 16; i += 2) {
     const float2 f = sm100::fmul2(make_float2(ks[i], ks[i + 1]), make_float2(r.size, r.size));
@@ -645,12 +656,14 @@ __device__ __forceinline__ void k8_softmax(const Kv8Attn& a, K8Rows& r, float (&
 
 // Scores of 64 keys in a stage of the ring, as joined integers.
 template <int NB>
-__device__ __forceinline__ void k8_scores(const uint8_t* stage, const K8Rows (&r)[NB], const uint32_t (&high)[4][4], const uint32_t (&zero)[4], float (&s)[NB][16], int gr, int c) {
+__device__ __forceinline__ void k8_scores(const uint8_t* stage, const K8Rows (&r)[NB], const uint32_t (&high)[4][4], const uint32_t (&zero)[4],
+                                          float (&s)[NB][16], int gr, int c) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     uint32_t k[8];
     const uint8_t* row = stage + (8 * j + gr) * 128;                   // row & 7 = gr
-    const uint4 x = *reinterpret_cast<const uint4*>(row + (((2 * c) ^ gr) << 4)), y = *reinterpret_cast<const uint4*>(row + (((2 * c + 1) ^ gr) << 4));
+    const uint4 x = *reinterpret_cast<const uint4*>(row + (((2 * c) ^ gr) << 4));
+    const uint4 y = *reinterpret_cast<const uint4*>(row + (((2 * c + 1) ^ gr) << 4));
     k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w, k[4] = y.x, k[5] = y.y, k[6] = y.z, k[7] = y.w;
     int lm[NB][4], hi[4];
 #pragma unroll
@@ -671,7 +684,8 @@ __device__ __forceinline__ void k8_scores(const uint8_t* stage, const K8Rows (&r
 // Adds 64 keys' weighted values.  A lane reads columns 16 g + 8 (half ^ (g >> 1 & 1)) .. of its keys at a time, so that no two lanes meet
 // in a bank; acc[8 half + x] are columns 32 c + 8 (half ^ (c & 1)) + x and that + 16.
 template <int NB>
-__device__ __forceinline__ void k8_values(const uint8_t* stage, const K8Weights (&w)[NB], const uint32_t (&high)[2][4], const uint32_t (&zero)[4], float2 (&acc)[NB][16], int gr, int c) {
+__device__ __forceinline__ void k8_values(const uint8_t* stage, const K8Weights (&w)[NB], const uint32_t (&high)[2][4], const uint32_t (&zero)[4],
+                                          float2 (&acc)[NB][16], int gr, int c) {
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     uint2 v[16];
@@ -735,7 +749,8 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     const long long per = (long long)a.H * a.c.dv;
     for (long long i = min(max(a.cu[a.n_seq], 0), a.n) * per + threadIdx.x; i < a.n * per; i += kK8Threads) out[i] = from_f<T>(0.f);
   }
-  const int hg = blockIdx.x % hs, share = blockIdx.x / hs, g = hg / groups, h0 = g * rep + hg % groups * kK8Heads, nh = min(kK8Heads, (g + 1) * rep - h0);
+  const int hg = blockIdx.x % hs, share = blockIdx.x / hs, g = hg / groups, h0 = g * rep + hg % groups * kK8Heads;
+  const int nh = min(kK8Heads, (g + 1) * rep - h0);
   int x = share, q0 = 0, left = 0x7fffffff, all = 0, shares = 1;
   if (a.cut) {
     // where the share begins: a lane counts the quanta of its tiles, and walks them if it is there; every warp for itself, without a barrier
@@ -877,8 +892,12 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       for (int b = 0; b < NB; ++b) k8_softmax(a, r[b], s[b], ks, vs, key0, c, key0 + kK8Keys > seen_by_all || key0 < seen_from, w[b]);
       failed = !sm100::mbar_wait_warp(&ring.full[warp][taken % kStages], (taken / kStages) & 1, gave_up);
       if (failed) break;
-      const uint32_t high[2][4] = {{w[0].high[0][0], NB == 2 ? w[NB - 1].high[0][0] : none[0], w[0].high[0][1], NB == 2 ? w[NB - 1].high[0][1] : none[1]},
-                                   {w[0].high[1][0], NB == 2 ? w[NB - 1].high[1][0] : none[2], w[0].high[1][1], NB == 2 ? w[NB - 1].high[1][1] : none[3]}};
+      uint32_t high[2][4];
+#pragma unroll
+      for (int y = 0; y < 8; ++y) {
+        const int z = y >> 2, half = y >> 1 & 1;
+        high[z][y & 3] = !(y & 1) ? w[0].high[z][half] : NB == 2 ? w[NB - 1].high[z][half] : none[y >> 1];
+      }
       k8_values<NB>(stages + taken % kStages * kK8Stage, w, high, zero, acc, gr, c);
       sm100::fence_proxy_async_smem();
       __syncwarp();
@@ -914,7 +933,8 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     float* slot = whole ? nullptr : a.part + ((size_t)blockIdx.x * 2 + (began == 0)) * R * LD;
     if (!whole && began == 0 && threadIdx.x == 0) {    // its last quantum is the share's of which the first is not behind it
       const long long last = k8_share(share + 1, all, shares) + behind - 1ll;
-      reinterpret_cast<K8Cut*>(a.part + (size_t)gridDim.x * 2 * R * LD)[blockIdx.x] = K8Cut{r0, n_rows, h0, nh, (int)(((last + 1) * shares - 1) / all) - share};
+      const int more_shares = (int)(((last + 1) * shares - 1) / all) - share;
+      reinterpret_cast<K8Cut*>(a.part + (size_t)gridDim.x * 2 * R * LD)[blockIdx.x] = K8Cut{r0, n_rows, h0, nh, more_shares};
     }
     const float* from[4];
     const float2* stats[4];
@@ -1133,9 +1153,9 @@ ELL_API int ell_kv8_append(const Kv8AppendCall* call, cudaStream_t stream) {
   const long long blocks = (x.max_new + 2 * x.c.block - 2) / x.c.block, ctas = (x.n_seq * blocks * 2 * c.G + 7) / 8;
   if (ctas > 0x0fffffff) return -2;
   const bool vec = c.d % 8 == 0 && c.dv % 8 == 0 && x.ldk * esz % 16 == 0 && x.ldv * esz % 16 == 0 && aligned_to(x.k, 16) && aligned_to(x.v, 16);
-#define ELL_APPEND(T, V)                                                                                                                              \
-  launch_chained(kv8_append_kernel<T, V>, (unsigned)ctas, 256, 0, stream, c, (const T*)x.k, (const T*)x.v, x.base, x.len, x.cu, (int)x.n_seq,          \
-                 (int)x.n, (int)blocks, (int)x.ldk, (int)x.ldv, x.err)
+#define ELL_APPEND(T, V)                                                                                                                \
+  launch_chained(kv8_append_kernel<T, V>, (unsigned)ctas, 256, 0, stream, c, (const T*)x.k, (const T*)x.v, x.base, x.len, x.cu,         \
+                 (int)x.n_seq, (int)x.n, (int)blocks, (int)x.ldk, (int)x.ldv, x.err)
   if (x.is_bf16) vec ? ELL_APPEND(__nv_bfloat16, 8) : ELL_APPEND(__nv_bfloat16, 1);
   else vec ? ELL_APPEND(float, 8) : ELL_APPEND(float, 1);
 #undef ELL_APPEND
@@ -1154,9 +1174,9 @@ ELL_API int ell_kv8_read(const Kv8ReadCall* call, cudaStream_t stream) {
   const long long most = x.n * x.max_len / (8 * kNumSMs) + 1;
   const int chunk = (int)std::max<long long>(beside, std::min<long long>(16 * beside, most / beside * beside));
   const dim3 grid((unsigned)((x.max_len + chunk - 1) / chunk), (unsigned)x.n);
-#define ELL_READ(T, V)                                                                                                                             \
-  launch_chained(kv8_read_kernel<T, V>, grid, 256, 0, stream, c, (T*)x.k, (T*)x.v, x.base, x.len, x.cu, x.row_base, (int)x.rows_q, (int)x.max_len, chunk, \
-                 x.err)
+#define ELL_READ(T, V)                                                                                                                  \
+  launch_chained(kv8_read_kernel<T, V>, grid, 256, 0, stream, c, (T*)x.k, (T*)x.v, x.base, x.len, x.cu, x.row_base, (int)x.rows_q,      \
+                 (int)x.max_len, chunk, x.err)
   if (x.is_bf16) vec == 8 ? ELL_READ(__nv_bfloat16, 8) : ELL_READ(__nv_bfloat16, 1);
   else vec == 8 ? ELL_READ(float, 8) : ELL_READ(float, 1);
 #undef ELL_READ
@@ -1177,14 +1197,17 @@ ELL_API int ell_attn_kv8(const Kv8AttnCall* call, cudaStream_t stream) {
   const Kv8AttnCall& x = *call;
   Kv8Attn a{};
   if (x.n <= 0) return 0;
-  if (!k8_cache(x.c, a.c) || x.n > 0x7fffffff || x.H <= 0 || x.H > 0x7fffff || x.H % x.c.G || x.max_len > 0x3fffffff || x.max_q > 0x3fffffff) return -2;
+  if (!k8_cache(x.c, a.c) || x.n > 0x7fffffff || x.H <= 0 || x.H > 0x7fffff || x.H % x.c.G) return -2;
+  if (x.max_len > 0x3fffffff || x.max_q > 0x3fffffff) return -2;
   const int n_seq = x.cu == nullptr ? 0 : (int)x.n_seq;
   const K8Plan p = k8_plan((int)x.n, n_seq, (int)x.max_q, (int)x.H, a.c.G, (int)x.max_len, (int)std::min(x.window, 0x3fffffffll));
   if (p.ctas <= 0) return -2;
   if (p.cut && (x.part == nullptr || !aligned_to(x.part, 16) || (size_t)x.part_floats < k8_part_floats(p))) return -2;
   a.q = x.q, a.out = x.out, a.part = x.part, a.base = x.base, a.len = x.len, a.cu = x.cu, a.sink = x.sink, a.slopes = x.slopes;
   a.n = (int)x.n, a.H = (int)x.H, a.ldq = (int)x.ldq, a.n_seq = n_seq, a.tiles = p.tiles, a.tt = p.tt, a.cut = p.cut;
-  a.window = x.window > 0 ? (int)std::min(x.window, 0x3fffffffll) : 0x3fffffff, a.scale = (float)(x.scale * 1.4426950408889634 / 2097152), a.err = x.err;
+  a.window = x.window > 0 ? (int)std::min(x.window, 0x3fffffffll) : 0x3fffffff;
+  a.scale = (float)(x.scale * 1.4426950408889634 / 2097152);
+  a.err = x.err;
   CUtensorMap tk, tv;
   int rc = make_tmap_bytes_heads(&tk, a.c.k, k8_row(a.c.d), a.c.G, a.c.rows, kK8Keys);
   if (!rc) rc = make_tmap_bytes_heads(&tv, a.c.v, k8_row(a.c.dv), a.c.G, a.c.rows, kK8Keys);

@@ -283,7 +283,8 @@ def attention_rows(q, k, v, base, length, max_len, scale, sink=None, alibi_slope
 # ---- a cache held in 8 bits ------------------------------------------------------------------------
 # A decoding step calls these for every layer, and a short context's kernels take less time than a call from Python: the arguments go over
 # as the words of one structure (csrc/kv8.cu), nine of which are the cache's.
-_KV8_CALLS = {"ell_kv8_append": struct.Struct("9q 5q 7q").pack, "ell_kv8_read": struct.Struct("9q 6q 5q").pack, "ell_attn_kv8": struct.Struct("9q 9q 9q d").pack}
+_KV8_CALLS = {"ell_kv8_append": struct.Struct("9q 5q 7q").pack, "ell_kv8_read": struct.Struct("9q 6q 5q").pack,
+              "ell_attn_kv8": struct.Struct("9q 9q 9q d").pack}
 _KV8_FNS, _ERR_WORDS = {}, {}
 
 
@@ -328,8 +329,8 @@ def _is_bf(dtype):
 
 @_on_device
 def kv8_append(k, v, words, base, length, cu_seqlens, max_new):
-    _kv8_call("ell_kv8_append", "kv8_append", 1, *words, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(), k.shape[0],
-              cu_seqlens.numel() - 1, max_new, _packed(k, "k"), _packed(v, "v"), _is_bf(k.dtype), _err_word(k.device))
+    _kv8_call("ell_kv8_append", "kv8_append", 1, *words, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(),
+              k.shape[0], cu_seqlens.numel() - 1, max_new, _packed(k, "k"), _packed(v, "v"), _is_bf(k.dtype), _err_word(k.device))
 
 
 @_on_device
@@ -337,15 +338,16 @@ def kv8_read(base, length, words, max_len, dtype):
     n, G, d, dv, dev = base.numel(), words[4], words[5], words[6], base.device
     k = torch.empty((n, max_len, G, d), dtype=dtype, device=dev)
     v = torch.empty_like(k) if d == dv else k.new_empty((n, max_len, G, dv))
-    _kv8_call("ell_kv8_read", "kv8_read", 1, *words, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), 0, 0, n, n, max_len, _is_bf(dtype),
-              _err_word(dev))
+    _kv8_call("ell_kv8_read", "kv8_read", 1, *words, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), 0, 0, n, n, max_len,
+              _is_bf(dtype), _err_word(dev))
     return k, v
 
 
-# Continued prompts with many rows (tokens times query heads of a key head): the cache's rows are written out in bf16 once and the tcgen05 kernel
-# attends to those, while that takes no more memory than this.  Us of the integer products on the cache | of rows read back (sequences, keys,
-# query and key heads, rows): 1 of 4096, 32/8, 128 rows 29 | 31, 256 43 | 37, 512 69 | 51, 2048 219 | 108; 1 of 4096, 32/32, 128 70 | 74, 256 123 |
-# 100; 1 of 30000, 64/8, 128 108 | 91, 256 195 | 126; 8 of 2000, 32/8, 256 58 | 67, 512 102 | 107, 1024 192 | 120; 2 of 400, 32/8, 256 21 | 27, 512 29 | 27.
+# Continued prompts with many rows (tokens times query heads of a key head): the cache's rows are written out in bf16 once and the tcgen05
+# kernel attends to those, while that takes no more memory than this.  Us of the integer products on the cache | of rows read back
+# (sequences, keys, query and key heads, rows): 1 of 4096, 32/8, 128 rows 29 | 31, 256 43 | 37, 512 69 | 51, 2048 219 | 108; 1 of 4096, 32/32,
+# 128 70 | 74, 256 123 | 100; 1 of 30000, 64/8, 128 108 | 91, 256 195 | 126; 8 of 2000, 32/8, 256 58 | 67, 512 102 | 107, 1024 192 | 120;
+# 2 of 400, 32/8, 256 21 | 27, 512 29 | 27.
 KV8_READ_ROWS, KV8_READ_LONG, KV8_READ_BYTES = 512, (256, 4096), 1 << 30
 KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 1024, 296, 4232
 
@@ -354,8 +356,8 @@ def _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slo
     T, n, G, dev = q.shape[0], cu_seqlens.numel() - 1, words[4], q.device
     k, v = (torch.empty(n * max_len, G, w, dtype=q.dtype, device=dev) for w in words[5:7])
     rows = torch.empty(2, T, dtype=torch.int32, device=dev)
-    _kv8_call("ell_kv8_read", "kv8_read", 1, *words, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(), rows.data_ptr(), n,
-              T, max_len, _is_bf(q.dtype), _err_word(dev))
+    _kv8_call("ell_kv8_read", "kv8_read", 1, *words, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(),
+              rows.data_ptr(), n, T, max_len, _is_bf(q.dtype), _err_word(dev))
     out = attention_rows(q, k, v, rows[0], rows[1], max_len, scale, sink, alibi_slopes, window, None, cu_seqlens, max_q)
     _check(lib().ell_kv8_clear(_p(out), _p(length), _p(cu_seqlens), c_int(n), c_int(T), c_int(out.shape[1] * out.shape[2]), _stream()), "kv8_clear")
     return out
@@ -367,18 +369,18 @@ def attention_kv8(q, words, base, length, max_len, scale, sink, alibi_slopes, wi
     window = window or 0
     n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, max_q)
     rows = max_q * (H // G)
-    if (rows >= KV8_READ_ROWS or (rows >= KV8_READ_LONG[0] and max_len >= KV8_READ_LONG[1])) and q.dtype is torch.bfloat16 and not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4) and \
-            2 * n_seq * max_len * G * (d + dv) <= KV8_READ_BYTES:
+    if (rows >= KV8_READ_ROWS or (rows >= KV8_READ_LONG[0] and max_len >= KV8_READ_LONG[1])) and q.dtype is torch.bfloat16 and \
+            not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4) and 2 * n_seq * max_len * G * (d + dv) <= KV8_READ_BYTES:
         return _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
     out = q.new_empty((T, H, dv))
     # room for what shares cut: a call has no more CTAs than are resident, or a CTA for each key head and 16 of its query heads
     need = max(KV8_CTAS, G * -(-(H // G) // 16)) * KV8_CTA_FLOATS if max_len > KV8_UNCUT else 0
     part = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
     sl = None if alibi_slopes is None else cu._slopes(alibi_slopes, H, q.device)
-    _kv8_call("ell_attn_kv8", "attn_kv8", 2 if need else 1, *words, q.data_ptr(), out.data_ptr(), 0 if part is None else part.data_ptr(), need, base.data_ptr(),
-              length.data_ptr(), 0 if sink is None else _f32(sink, "sink").data_ptr(), 0 if sl is None else sl.data_ptr(),
-              0 if cu_seqlens is None else cu_seqlens.data_ptr(), T, n_seq, max_q, H, _packed(q, "q"), max_len, window, _is_bf(q.dtype), _err_word(q.device),
-              scale)
+    _kv8_call("ell_attn_kv8", "attn_kv8", 2 if need else 1, *words, q.data_ptr(), out.data_ptr(), 0 if part is None else part.data_ptr(), need,
+              base.data_ptr(), length.data_ptr(), 0 if sink is None else _f32(sink, "sink").data_ptr(), 0 if sl is None else sl.data_ptr(),
+              0 if cu_seqlens is None else cu_seqlens.data_ptr(), T, n_seq, max_q, H, _packed(q, "q"), max_len, window, _is_bf(q.dtype),
+              _err_word(q.device), scale)
     return out
 
 

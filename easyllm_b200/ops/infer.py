@@ -243,9 +243,10 @@ KV8_MOST = 128          # head sizes, and rows that share a scale
 class KV8(NamedTuple):
     """Keys and values of the cache rows of a layer in 8 bits: k ``[R, G, dim]``, v ``[R, G, vdim]`` int8 with head sizes padded to
     multiples of 16, and for each block of rows and head a scale, k_scale / v_scale ``[R / block, G]`` fp32 (``block``: a power of two up to
-    128).  A value is ``int8 * scale``.  Scales are powers of two, the least of which 127 times is the block's largest magnitude or more (at most 2^121: larger values become 127 times that), so
-    that nothing but the rounding to 8 bits is ever lost: values are exact in bf16 and fp32, and in a block that rows join one by one they
-    are off by less than one scale.  Where a block got a value that is not finite, it reads as NaN."""
+    128).  A value is ``int8 * scale``.  Scales are powers of two, the least of which 127 times is the block's largest magnitude or more (at most
+    2^121: larger values become 127 times that), so that nothing but the rounding to 8 bits is ever lost: values are exact in bf16 and fp32,
+    and in a block that rows join one by one they are off by less than one scale.  Where a block got a value that is not finite, it reads as
+    NaN."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
@@ -288,8 +289,9 @@ def _kv8_check(cache, *ints):
 def kv8_append(cache, k, v, meta):
     """Quantise the step's keys k ``[T, G, dim]`` and values v ``[T, G, vdim]`` into their places of ``cache``: the rows between two borders
     of ``meta["cu_seqlens"]`` are the next tokens of one sequence, of which the first goes to row ``kv_base + kv_len - 1`` (a sequence starts
-    at a block; the sequences of a step are distinct).  ``meta["max_seqlen"]`` bounds their numbers.  Rows behind the last border, and sequences whose ``kv_len`` is 0, are left out.
-    A block that has rows already keeps the larger scale; if that is the new one, its rows are rounded again."""
+    at a block; the sequences of a step are distinct).  ``meta["max_seqlen"]`` bounds their numbers.  Rows behind the last border, and sequences
+    whose ``kv_len`` is 0, are left out.  A block that has rows already keeps the larger scale; if that is the new one, its rows are rounded
+    again."""
     no_grad_check(k, v)
     base, length, cu = meta["kv_base"], meta["kv_len"], meta["cu_seqlens"]
     words = _kv8_check(cache, base, length, cu)
