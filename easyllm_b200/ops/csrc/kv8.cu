@@ -72,10 +72,11 @@ struct K8Elems<__nv_bfloat16, 8> {
   __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ float amax(float m) const {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m = max3_nan(m, __uint_as_float((w[i] & 0x7fffu) << 16), __uint_as_float(w[i] & 0x7fff0000u));
-    return m;
+    const uint32_t w[4] = {u.x & 0x7fff7fffu, u.y & 0x7fff7fffu, u.z & 0x7fff7fffu, u.w & 0x7fff7fffu};
+    const __nv_bfloat162 a = __hmax2_nan(reinterpret_cast<const __nv_bfloat162&>(w[0]), reinterpret_cast<const __nv_bfloat162&>(w[1]));
+    const __nv_bfloat162 b = __hmax2_nan(reinterpret_cast<const __nv_bfloat162&>(w[2]), reinterpret_cast<const __nv_bfloat162&>(w[3]));
+    const float2 f = __bfloat1622float2(__hmax2_nan(a, b));
+    return max3_nan(m, f.x, f.y);
   }
   template <bool TOP>
   __device__ __forceinline__ void store(int8_t* dst, float inv) const {
@@ -122,11 +123,11 @@ struct K8Elems<T, 1> {
 template <typename T, int V>
 __global__ void __launch_bounds__(256, 4)
 kv8_append_kernel(const Kv8Cache c, const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ base_, const int* __restrict__ len_,
-                  const int* __restrict__ cu, int n_seq, int n, int blocks, int ldk, int ldv, int* __restrict__ err) {
+                  const int* __restrict__ cu, int n, int blocks, int ldk, int ldv, int* __restrict__ err) {
   chain_enter(k, v, base_, len_, cu, err);
-  const unsigned item = blockIdx.x * 8u + (threadIdx.x >> 5), rest = item / c.G;
-  const int lane = threadIdx.x & 31, g = (int)(item % c.G), which = (int)(rest & 1), j = (int)((rest >> 1) % blocks), s = (int)((rest >> 1) / blocks);
-  if (s >= n_seq) return;
+  const unsigned wide = 2u * c.G, across = (wide + 7) / 8, j = blockIdx.x / across, item = (blockIdx.x - j * across) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, which = item >= (unsigned)c.G, g = (int)item - which * c.G, s = blockIdx.y;
+  if (item >= wide) return;
   const int r0 = cu[s], count = min(cu[s + 1], n) - r0;
   if (count <= 0 || r0 < 0) return;
   const int base = base_[r0], p0 = len_[r0] - 1;
@@ -135,9 +136,9 @@ kv8_append_kernel(const Kv8Cache c, const T* __restrict__ k, const T* __restrict
     if (lane == 0) atomicCAS(err, 0, kK8Place);
     return;
   }
-  const int b = (p0 >> c.shift) + j, start = b << c.shift, first = max(p0, start), last = min(p0 + count, start + (1 << c.shift));
+  const int b = (p0 >> c.shift) + (int)j, start = b << c.shift, first = max(p0, start), last = min(p0 + count, start + (1 << c.shift));
   if (first >= last) return;
-  if (lane == 0 && j == blocks - 1 && last < p0 + count) atomicCAS(err, 0, kK8Place);      // more rows than was said: they are left out
+  if (lane == 0 && (int)j == blocks - 1 && last < p0 + count) atomicCAS(err, 0, kK8Place);      // more rows than was said: they are left out
   const int width = which ? c.dv : c.d, row = k8_row(width), step = c.G * row, rows = last - first;
   const size_t ld = which ? ldv : ldk;
   const T* src = (which ? v : k) + (size_t)(r0 + first - p0) * ld + (size_t)g * width;
@@ -188,7 +189,7 @@ kv8_append_kernel(const Kv8Cache c, const T* __restrict__ k, const T* __restrict
     }
   }
   const bool none = now != now, top = now == k8_scale_of(3.4028235e38f);
-  const float inv = none ? 0.f : 1.f / now;                       // a power of two
+  const float inv = none ? 0.f : __uint_as_float(0x7f000000u - __float_as_uint(now));      // of a power of two
   for (int x = 0; x < turns; ++x)
     for (int r = 0; r < rows; r += chunk) {
       const int at = x * 32 + piece * V;
@@ -248,9 +249,10 @@ __device__ __forceinline__ void k8_store_values(T* o, const uint32_t* w, float s
 // row_base[r] becomes the place of a query row's keys in ko, row_base[rows + r] its length, max_len at most.  A thread keeps its place in a row, V
 // elements, and takes positions, eight of which are under way together.  Bound by memory: 8 prefixes of up to 4096 rows, 8 heads of 128 (37 MB
 // in, 134 MB out, zeros among them) 31 us, 5.5 TB/s.  With a division for every eight values it took 48 us, with conversions of the integers
-// 39, with 16 values a thread, whose stores leave every other 16 bytes to the next one, 134.
+// 39, with 16 values a thread, whose stores leave every other 16 bytes to the next one, 134.  One prompt of 4096 rows of 32 heads 18.5 us; 27 where
+// a CTA took four positions of whole rows.
 template <typename T, int V>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 kv8_read_kernel(const Kv8Cache c, T* __restrict__ ko, T* __restrict__ vo, const int* __restrict__ base, const int* __restrict__ len,
                 const int* __restrict__ cu, int* __restrict__ row_base, int rows, int max_len, int chunk, int* __restrict__ err) {
   chain_enter(ko, vo, base, len, cu, row_base, err);
@@ -260,7 +262,7 @@ kv8_read_kernel(const Kv8Cache c, T* __restrict__ ko, T* __restrict__ vo, const 
     r0 = cu[i];
     r1 = min(cu[i + 1], rows);
     if (r0 < 0 || r0 >= r1) return;
-    if (blockIdx.x == 0)
+    if (blockIdx.x == 0 && blockIdx.z == 0)
       for (int r = r0 + threadIdx.x; r < r1; r += 256) {
         row_base[r] = i * max_len;
         row_base[rows + r] = min(len[r], max_len);
@@ -271,7 +273,8 @@ kv8_read_kernel(const Kv8Cache c, T* __restrict__ ko, T* __restrict__ vo, const 
   if ((!ok || (cu != nullptr && len[r1 - 1] > max_len)) && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(err, 0, kK8Place);
   const int p0 = blockIdx.x * chunk, p1 = min(p0 + chunk, cu != nullptr && ok ? n : max_len);
   const int beside = max(1, 256 / per);                          // positions that the threads take side by side
-  for (int y = threadIdx.x; y < beside * per; y += 256) {
+  const int y = blockIdx.z * 256 + threadIdx.x;
+  if (y < beside * per) {
     const int z0 = y % per, at_p = y / per;
     const bool is_v = z0 >= c.G * pk;
     const int z = is_v ? z0 - c.G * pk : z0, pieces = is_v ? pv : pk, width = is_v ? c.dv : c.d, row = k8_row(width);
@@ -1150,12 +1153,12 @@ ELL_API int ell_kv8_append(const Kv8AppendCall* call, cudaStream_t stream) {
   if (x.n <= 0 || x.n_seq <= 0 || x.max_new <= 0) return 0;
   if (!k8_cache(x.c, c) || x.n > 0x7fffffff) return -2;
   const int esz = x.is_bf16 ? 2 : 4;
-  const long long blocks = (x.max_new + 2 * x.c.block - 2) / x.c.block, ctas = (x.n_seq * blocks * 2 * c.G + 7) / 8;
-  if (ctas > 0x0fffffff) return -2;
+  const long long blocks = (x.max_new + 2 * x.c.block - 2) / x.c.block, ctas = blocks * ((2 * c.G + 7) / 8);
+  if (ctas > 0x7fffffff || x.n_seq > 65535) return -2;
   const bool vec = c.d % 8 == 0 && c.dv % 8 == 0 && x.ldk * esz % 16 == 0 && x.ldv * esz % 16 == 0 && aligned_to(x.k, 16) && aligned_to(x.v, 16);
 #define ELL_APPEND(T, V)                                                                                                                \
-  launch_chained(kv8_append_kernel<T, V>, (unsigned)ctas, 256, 0, stream, c, (const T*)x.k, (const T*)x.v, x.base, x.len, x.cu,         \
-                 (int)x.n_seq, (int)x.n, (int)blocks, (int)x.ldk, (int)x.ldv, x.err)
+  launch_chained(kv8_append_kernel<T, V>, dim3((unsigned)ctas, (unsigned)x.n_seq), 256, 0, stream, c, (const T*)x.k, (const T*)x.v,      \
+                 x.base, x.len, x.cu, (int)x.n, (int)blocks, (int)x.ldk, (int)x.ldv, x.err)
   if (x.is_bf16) vec ? ELL_APPEND(__nv_bfloat16, 8) : ELL_APPEND(__nv_bfloat16, 1);
   else vec ? ELL_APPEND(float, 8) : ELL_APPEND(float, 1);
 #undef ELL_APPEND
@@ -1169,11 +1172,10 @@ ELL_API int ell_kv8_read(const Kv8ReadCall* call, cudaStream_t stream) {
   if (x.n <= 0 || x.max_len <= 0) return 0;
   if (!k8_cache(x.c, c) || x.n > 65535 || x.max_len > 0x3fffffff || (x.cu != nullptr && x.n * x.max_len > 0x7fffffff)) return -2;
   const int vec = c.d % 8 == 0 && c.dv % 8 == 0 ? 8 : 1;
-  // positions of a CTA: sixteen turns of its threads, fewer where that leaves SMs without work
-  const int per = c.G * (c.d + c.dv) / vec, beside = std::max(1, 256 / per);
-  const long long most = x.n * x.max_len / (8 * kNumSMs) + 1;
-  const int chunk = (int)std::max<long long>(beside, std::min<long long>(16 * beside, most / beside * beside));
-  const dim3 grid((unsigned)((x.max_len + chunk - 1) / chunk), (unsigned)x.n);
+  // a thread takes eight positions (with sixteen or thirty-two the 31 us beside kv8_read_kernel become 32 and 35)
+  const int per = c.G * (c.d + c.dv) / vec, beside = std::max(1, 256 / per), z = (beside * per + 255) / 256, chunk = 8 * beside;
+  if (z > 65535) return -2;
+  const dim3 grid((unsigned)((x.max_len + chunk - 1) / chunk), (unsigned)x.n, (unsigned)z);
 #define ELL_READ(T, V)                                                                                                                  \
   launch_chained(kv8_read_kernel<T, V>, grid, 256, 0, stream, c, (T*)x.k, (T*)x.v, x.base, x.len, x.cu, x.row_base, (int)x.rows_q,      \
                  (int)x.max_len, chunk, x.err)

@@ -238,6 +238,7 @@ def attention_rows(q, k, v, kv_base, kv_len, max_len, scale, sink=None, alibi_sl
 
 # ---- a cache held in 8 bits -------------------------------------------------------------------------
 KV8_MOST = 128          # head sizes, and rows that share a scale
+KV8_SEQUENCES = 65535   # of a call that writes or reads
 
 
 class KV8(NamedTuple):
@@ -297,8 +298,9 @@ def kv8_append(cache, k, v, meta):
     words = _kv8_check(cache, base, length, cu)
     T, G = k.shape[0], words[4]
     if k.shape != (T, G, words[5]) or v.shape != (T, G, words[6]) or k.dtype != v.dtype or not k.get_device() == v.get_device() == base.get_device() or \
-            base.numel() != T or length.numel() != T or cu.numel() < 1:
-        raise ValueError(f"kv8_append: k [T, {G}, {cache.dim}] and v [T, {G}, {cache.vdim}] of one dtype, a place and a length for each row")
+            base.numel() != T or length.numel() != T or not 1 <= cu.numel() <= KV8_SEQUENCES + 1:
+        raise ValueError(f"kv8_append: k [T, {G}, {cache.dim}] and v [T, {G}, {cache.vdim}] of one dtype, a place and a length for each row, and "
+                         f"the borders of up to {KV8_SEQUENCES} sequences")
     if _kern(k):
         return _cu().kv8_append(k, v, words, base, length, cu, meta["max_seqlen"])
     ref.kv8_append(cache, k, v, meta)
@@ -308,8 +310,8 @@ def kv8_read(cache, kv_base, kv_len, max_len, dtype=torch.bfloat16):
     """The values of ``cache`` as keys ``[n, max_len, G, dim]`` and values ``[n, max_len, G, vdim]``: for each sequence the rows ``kv_base`` ..
     ``kv_base + kv_len`` (at most ``max_len``), then zeros.  Exact in bf16 and fp32."""
     words = _kv8_check(cache, kv_base, kv_len)
-    if kv_base.shape != kv_len.shape or dtype not in (torch.bfloat16, torch.float32) or max_len < 0:
-        raise ValueError("kv8_read: a place and a length for each sequence, into bf16 or fp32")
+    if kv_base.shape != kv_len.shape or kv_base.numel() > KV8_SEQUENCES or dtype not in (torch.bfloat16, torch.float32) or max_len < 0:
+        raise ValueError(f"kv8_read: a place and a length for each of up to {KV8_SEQUENCES} sequences, into bf16 or fp32")
     if cache.k.is_cuda:
         return _cu().kv8_read(kv_base, kv_len, words, max_len, dtype)
     return ref.kv8_read(cache, kv_base, kv_len, max_len, dtype)

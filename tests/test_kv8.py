@@ -423,6 +423,10 @@ def test_refusals():
     with pytest.raises(ValueError):
         iops.kv8_append(cache, k, v, dict(meta, cu_seqlens=ints([])))
     with pytest.raises(ValueError):
+        iops.kv8_append(cache, k, v, dict(meta, cu_seqlens=torch.ones(65537, dtype=torch.int32)))
+    with pytest.raises(ValueError):
+        iops.kv8_read(cache, torch.zeros(65536, dtype=torch.int32), torch.zeros(65536, dtype=torch.int32), 4)
+    with pytest.raises(ValueError):
         iops.kv8_read(cache, one, one, 4, torch.float16)
     with pytest.raises(RuntimeError):
         iops.attention_kv8(**{**ok, "q": q.clone().requires_grad_()})
