@@ -1195,12 +1195,14 @@ ELL_API int ell_kv8_clear(void* out, const int* len, const int* cu, int n_seq, i
 // q rows of ldq elements.  max_len bounds len[].  part (16-byte aligned): `part_floats` of scratch where max_len is above 1024, enough for
 // max(296, key heads x groups of 16 query heads) x 4232.  window: keys a row sees (<= 0: all).  cu [n_seq + 1] (or null): rows
 // cu[i] .. cu[i + 1] - 1 are consecutive tokens of one sequence, with one base and lengths that grow by one; max_q bounds their number.
+// There is one sequence at least where there are borders.
 ELL_API int ell_attn_kv8(const Kv8AttnCall* call, cudaStream_t stream) {
   const Kv8AttnCall& x = *call;
   Kv8Attn a{};
   if (x.n <= 0) return 0;
   if (!k8_cache(x.c, a.c) || x.n > 0x7fffffff || x.H <= 0 || x.H > 0x7fffff || x.H % x.c.G) return -2;
   if (x.max_len > 0x3fffffff || x.max_q > 0x3fffffff) return -2;
+  if (x.cu != nullptr && (x.n_seq <= 0 || x.n_seq > 0x7fffffff)) return -2;      // borders without a sequence: a tile would look behind them
   const int n_seq = x.cu == nullptr ? 0 : (int)x.n_seq;
   const K8Plan p = k8_plan((int)x.n, n_seq, (int)x.max_q, (int)x.H, a.c.G, (int)x.max_len, (int)std::min(x.window, 0x3fffffffll));
   if (p.ctas <= 0) return -2;

@@ -335,6 +335,8 @@ def attention_kv8(q, cache, kv_base, kv_len, max_len, scale, sink=None, alibi_sl
             raise ValueError(f"attention_kv8: {name} has one value for each of the {H} heads on their device")
     if cu_seqlens is not None and (max_q is None or cu_seqlens.numel() < 1):
         raise ValueError("attention_kv8: cu_seqlens has a border at least, and comes with max_q, a bound of the sequences' rows")
+    if cu_seqlens is not None and cu_seqlens.numel() == 1:         # no sequence: every row is behind the last border
+        return q.new_zeros(T, H, words[6])
     if _kern(q):
         return _cu().attention_kv8(q, words, kv_base, kv_len, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
     return ref.attention_kv8(q, cache, kv_base, kv_len, scale, sink, alibi_slopes, window, cu_seqlens)
