@@ -246,7 +246,8 @@ __device__ __forceinline__ void k8_store_values(T* o, const uint32_t* w, float s
 }
 // ko [n, max_len, G, d], vo [n, max_len, G, dv].  cu null: rows base[i] .. base[i] + len[i] - 1 of the cache, then zeros.  Otherwise sequence i has
 // the query rows cu[i] .. cu[i + 1] - 1 with base and len of their own: its rows are those that its last one sees, nothing is written behind them,
-// row_base[r] becomes the place of a query row's keys in ko, row_base[rows + r] its length, max_len at most.  A thread keeps its place in a row, V
+// row_base[r] becomes the place of a query row's keys in ko, row_base[rows + r] its length, max_len at most; both are 0 for rows behind the
+// last sequence.  A thread keeps its place in a row, V
 // elements, and takes positions, eight of which are under way together.  Bound by memory: 8 prefixes of up to 4096 rows, 8 heads of 128 (37 MB
 // in, 134 MB out, zeros among them) 31 us, 5.5 TB/s.  With a division for every eight values it took 48 us, with conversions of the integers
 // 39, with 16 values a thread, whose stores leave every other 16 bytes to the next one, 134.  One prompt of 4096 rows of 32 heads 18.5 us; 27 where
@@ -261,6 +262,8 @@ kv8_read_kernel(const Kv8Cache c, T* __restrict__ ko, T* __restrict__ vo, const 
   if (cu != nullptr) {
     r0 = cu[i];
     r1 = min(cu[i + 1], rows);
+    if (i == gridDim.y - 1 && blockIdx.x == 0 && blockIdx.z == 0)
+      for (int r = max(r1, 0) + threadIdx.x; r < rows; r += 256) row_base[r] = row_base[rows + r] = 0;
     if (r0 < 0 || r0 >= r1) return;
     if (blockIdx.x == 0 && blockIdx.z == 0)
       for (int r = r0 + threadIdx.x; r < r1; r += 256) {

@@ -344,7 +344,8 @@ def kv8_read(base, length, words, max_len, dtype):
 
 
 # Continued prompts with many rows (tokens times query heads of a key head): the cache's rows are written out in bf16 once and the tcgen05
-# kernel attends to those, while that takes no more memory than this.  Us of the integer products on the cache | of rows read back
+# kernel attends to those, while that takes no more memory than this.  That kernel goes by the borders of sequences of several tokens; single
+# ones, however many heads they have, stay on the cache's bytes.  Us of the integer products on the cache | of rows read back
 # (sequences, keys, query and key heads, rows): 1 of 4096, 32/8, 128 rows 29 | 31, 256 43 | 37, 512 69 | 51, 2048 219 | 108; 1 of 4096, 32/32,
 # 128 70 | 74, 256 123 | 100; 1 of 30000, 64/8, 128 108 | 91, 256 195 | 126; 8 of 2000, 32/8, 256 58 | 67, 512 102 | 107, 1024 192 | 120;
 # 2 of 400, 32/8, 256 21 | 27, 512 29 | 27.
@@ -369,7 +370,7 @@ def attention_kv8(q, words, base, length, max_len, scale, sink, alibi_slopes, wi
     window = window or 0
     n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, max_q)
     rows = max_q * (H // G)
-    if (rows >= KV8_READ_ROWS or (rows >= KV8_READ_LONG[0] and max_len >= KV8_READ_LONG[1])) and q.dtype is torch.bfloat16 and \
+    if max_q > 1 and (rows >= KV8_READ_ROWS or (rows >= KV8_READ_LONG[0] and max_len >= KV8_READ_LONG[1])) and q.dtype is torch.bfloat16 and \
             not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4) and 2 * n_seq * max_len * G * (d + dv) <= KV8_READ_BYTES:
         return _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
     out = q.new_empty((T, H, dv))

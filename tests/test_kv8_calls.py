@@ -45,3 +45,65 @@ def test_rows_without_a_sequence_are_zero(device, dtype, max_len, max_q, H):
     places = ints([0, 999, -1, 1 << 30, 16], dev)
     got = iops.attention_kv8(torch.ones(5, H, 32, dtype=dtype, device=dev), cache, places, places, max_len, 1.0, cu_seqlens=ints([0], dev), max_q=max_q)
     assert got.shape == (5, H, 32) and got.dtype == dtype and not bool(got.any())
+
+
+# ---- rows read back -----------------------------------------------------------------------------------
+def way(monkeypatch, T, H, cache, max_len, cu_seqlens, max_q, window=None, dtype=BF16):
+    """Which way a call takes on a GPU: "bytes" (integer products on the cache) or "back" (rows read back).  Nothing is launched."""
+    from easyllm_b200.ops import cuda_infer as ci
+    taken = []
+    monkeypatch.setattr(ci, "_attention_read_back", lambda *a: taken.append("back"))
+    monkeypatch.setattr(ci, "_kv8_call", lambda name, *a: taken.append("bytes"))
+    monkeypatch.setattr(ci, "_err_word", lambda device: 0)
+    places = ints([0] * T)
+    q = torch.empty(T, H, cache.dim, dtype=dtype)
+    ci.attention_kv8.__wrapped__(q, iops._kv8_check(cache, places), places, places, max_len, 1.0, None, None, window, cu_seqlens, max_q)
+    assert len(taken) == 1
+    return taken[0]
+
+
+def test_single_tokens_stay_on_the_bytes_whatever_their_heads(monkeypatch):
+    """The kernel behind the other way goes by borders of sequences of several tokens: without them, or with one token each, it takes every
+    row by its own place, also rows behind the last border, which have none."""
+    cache = iops.kv8_empty(64, 1, 128, 128, 16)
+    for H in (256, 512, 1024):
+        for max_len in (64, 5000):
+            assert way(monkeypatch, 3, H, cache, max_len, None, None) == "bytes"
+            assert way(monkeypatch, 3, H, cache, max_len, ints([0, 1, 2]), 1) == "bytes"
+            assert way(monkeypatch, 3, H, cache, max_len, ints([0, 2]), 2) == ("back" if 2 * H >= 512 else "bytes")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("device", ["cuda"])
+@pytest.mark.parametrize("H,longest,block", [(512, 90, 16), (256, 4200, 64), (512, 4200, 16), (258, 4200, 16)])
+def test_single_tokens_of_many_heads(device, H, longest, block):
+    """One key head for hundreds of query heads, as tokens of their own and as sequences of one, with rows behind the last border."""
+    dev = _device(device)
+    n, d, cap = 3, 32, -(-longest // 128) * 128
+    cache, plain = filled(n * cap, 1, d, d, block, dev)
+    q = rand(n + 2, H, d, seed=1).to(BF16).to(dev)
+    total = [longest, 1, longest // 2]
+    base, length = ints([0, cap, 2 * cap, 1 << 30, -7], dev), ints(total + [99, 1 << 30], dev)
+    alone = iops.attention_kv8(q[:n], cache, base[:n], length[:n], longest, 0.2)
+    bordered = iops.attention_kv8(q, cache, base, length, longest, 0.2, cu_seqlens=ints([0, 1, 2, 3], dev), max_q=1)
+    assert torch.equal(bordered[:n], alone) and not bool(bordered[n:].any())
+    for r, t in enumerate(total):
+        near(alone[r], *plain_attention(q[r], *(p.values(r * cap, t) for p in plain), 0.2))
+
+
+@pytest.mark.gpu
+def test_rows_behind_the_last_border_have_no_place_among_rows_read_back():
+    """What the attention over rows read back is told of them: place 0, length 0."""
+    from easyllm_b200.ops import cuda_infer as ci
+    dev = _device("cuda")
+    cache, _ = filled(512, 2, 32, 32, 16, dev)
+    for cu, rows in (([0, 3, 5], 9), ([0, 5, 5], 9), ([0, 5], 300), ([0, 0], 4), ([0, 9], 9)):
+        cu, max_len, n = ints(cu, dev), 64, len(cu) - 1
+        length, base = ints([40 + r for r in range(rows)], dev).clamp(max=64), ints([0] * rows, dev)
+        k, v = (torch.empty(n * max_len, 2, 32, dtype=BF16, device=dev) for _ in "kv")
+        place = torch.full((2, rows), -1, dtype=torch.int32, device=dev)
+        ci._kv8_call("ell_kv8_read", "kv8_read", 1, *iops._kv8_check(cache, cu), k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(),
+                     cu.data_ptr(), place.data_ptr(), n, rows, max_len, 1, ci._err_word(dev))
+        border = cu.tolist()
+        want = [[i * max_len for i in range(n) for _ in range(border[i + 1] - border[i])], length.tolist()[:border[-1]]]
+        assert place.tolist() == [w + [0] * (rows - border[-1]) for w in want]
