@@ -1141,7 +1141,7 @@ struct Kv8AttnCall {
 static_assert(sizeof(Kv8Args) == 9 * 8 && sizeof(Kv8AppendCall) == 21 * 8 && sizeof(Kv8ReadCall) == 20 * 8 && sizeof(Kv8AttnCall) == 28 * 8, "");
 static bool k8_cache(const Kv8Args& a, Kv8Cache& c) {
   const bool ok = a.G > 0 && a.G <= 65535 && a.d > 0 && a.dv > 0 && a.d <= kK8Dim && a.dv <= kK8Dim && a.block > 0 && a.block <= kK8MaxBlock &&
-                  !(a.block & (a.block - 1)) && a.rows % a.block == 0 && a.rows <= 0x7fffffff;
+                  !(a.block & (a.block - 1)) && a.rows % a.block == 0 && a.rows <= 0x7fffffff && aligned_to(a.k, 16) && aligned_to(a.v, 16);
   int shift = 0;
   while ((1ll << shift) < a.block) ++shift;
   c = Kv8Cache{a.k, a.v, a.ks, a.vs, a.rows, (int)a.G, (int)a.d, (int)a.dv, shift};

@@ -281,6 +281,8 @@ def _kv8_check(cache, *ints):
         raise ValueError("an 8-bit cache is contiguous: int8 [R, G, dim padded to 16] rows, fp32 [R / block, G] scales, blocks of a power of two")
     if not dev == v.get_device() == ks.get_device() == vs.get_device():
         raise ValueError("the parts of an 8-bit cache are on one device")
+    if (k.data_ptr() | v.data_ptr()) & 15:
+        raise ValueError("the rows of an 8-bit cache start on a 16-byte boundary: they are moved in pieces of up to 16 bytes")
     for t in ints:
         if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.get_device() != dev:
             raise ValueError("places and lengths of cache rows are contiguous int32 vectors on the cache's device")

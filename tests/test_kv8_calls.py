@@ -107,3 +107,68 @@ def test_rows_behind_the_last_border_have_no_place_among_rows_read_back():
         border = cu.tolist()
         want = [[i * max_len for i in range(n) for _ in range(border[i + 1] - border[i])], length.tolist()[:border[-1]]]
         assert place.tolist() == [w + [0] * (rows - border[-1]) for w in want]
+
+
+# ---- where the cache starts -----------------------------------------------------------------------------
+def shifted(cache, name, by):
+    """``cache`` with one of its tensors starting ``by`` bytes behind a 16-byte boundary, contiguous as before."""
+    t = getattr(cache, name)
+    room = torch.zeros(t.numel() * t.element_size() + 32, dtype=torch.uint8, device=t.device)
+    start = -room.data_ptr() % 16 + by
+    moved = room[start:start + t.numel() * t.element_size()].view(t.dtype).view(t.shape)
+    assert moved.data_ptr() % 16 == by and moved.is_contiguous()
+    moved.copy_(t)
+    return cache._replace(**{name: moved})
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("name,by", [("k", 1), ("k", 4), ("v", 8), ("v", 15)])
+def test_rows_that_start_off_a_boundary_are_refused(device, name, by):
+    dev = _device(device)
+    cache, one = shifted(iops.kv8_empty(64, 2, 32, 16, 16, dev), name, by), ints([0], dev)
+    with pytest.raises(ValueError, match="16-byte"):
+        iops.kv8_append(cache, torch.zeros(1, 2, 32, device=dev), torch.zeros(1, 2, 16, device=dev), step([1], [0], [0], 64, dev))
+    with pytest.raises(ValueError, match="16-byte"):
+        iops.kv8_read(cache, one, one, 4)
+    for dtype in (F32, BF16):
+        with pytest.raises(ValueError, match="16-byte"):
+            iops.attention_kv8(torch.zeros(1, 4, 32, dtype=dtype, device=dev), cache, one, one, 4, 1.0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("d,dv", [(32, 16), (40, 9)])
+def test_scales_and_inputs_may_start_anywhere(device, d, dv):
+    """Scales behind a 4-byte boundary, new rows and queries behind that of their type: the rows of an aligned cache, to the bit, and attention
+    over them within the bound of 32-bit sums (on the CPU a library's product, whose order of sums goes by where its operands start)."""
+    dev = _device(device)
+    T, G, H, cap = 37, 2, 4, 64
+    for dtype in (F32, BF16):
+        k, v, q = (rand(T * n * w + 1, seed=w + n).to(dtype).to(dev) for n, w in ((G, d), (G, dv), (H, d)))
+        results = []
+        for at in (0, 1):
+            cache = iops.kv8_empty(cap, G, d, dv, 16, dev)
+            if at:
+                cache = shifted(shifted(cache, "k_scale", 4), "v_scale", 12)
+            meta = step([T], [0], [0], cap, dev)
+            kk, vv, qq = (t[1:].view(T, n, w) if at else t[1:].clone().view(T, n, w) for t, n, w in ((k, G, d), (v, G, dv), (q, H, d)))
+            iops.kv8_append(cache, kk, vv, meta)
+            results.append(iops.kv8_read(cache, ints([0], dev), ints([T], dev), T, dtype))
+            got = iops.attention_kv8(qq, cache, meta["kv_base"], meta["kv_len"], T, 0.2, cu_seqlens=meta["cu_seqlens"], max_q=T)
+            rows = [x[0].double().cpu() for x in results[-1]]
+            for r in range(T):
+                near(got[r], *plain_attention(qq[r], *(x[:r + 1] for x in rows), 0.2))
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+
+
+def test_the_entries_refuse_rows_off_a_boundary():
+    """Before they look at anything on the device, so this needs none."""
+    import ctypes
+    from easyllm_b200.ops import cuda, cuda_infer
+    at = 1 << 20
+    rest = {"ell_kv8_append": (at, at, at, at, at, 1, 1, 1, 64, 32, 1, at), "ell_kv8_read": (at, at, at, at, 0, 0, 1, 1, 4, 1, at),
+            "ell_attn_kv8": (at, at, 0, 0, at, at, 0, 0, 0, 1, 0, 1, 4, 128, 4, 0, 1, at, 1.0)}
+    for name, words in rest.items():
+        for k, v in ((at + 1, at), (at, at + 8)):
+            call = cuda_infer._KV8_CALLS[name](k, v, at, at, 2, 32, 16, 16, 64, *words)
+            assert getattr(cuda.lib(), name)(ctypes.c_char_p(call), ctypes.c_void_p(0)) == -2, name
