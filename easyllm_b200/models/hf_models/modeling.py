@@ -165,6 +165,9 @@ def _layer_specs(cfg: dict, mixers, mlps) -> List[LayerSpec]:
     return layers
 
 
+_NO_HEADS = "kv_cache_block: latent attention keeps no keys and values of heads"
+
+
 def _megozen_arch(cfg: dict) -> HFArch:
     """``config.json`` of a Megozen model: vocab, width, norm.eps, embedding.bigram and one entry per layer."""
     layers = _layer_specs(cfg, ("latent_attention",), ("moe",))
@@ -176,7 +179,7 @@ def _megozen_arch(cfg: dict) -> HFArch:
         if window is not None and window < 1:
             raise ValueError(f"layer {i}: a window of {window} tokens")
     if cfg.get("kv_cache_block"):
-        raise ValueError("kv_cache_block: latent attention keeps no keys and values of heads")
+        raise ValueError(_NO_HEADS)
     return HFArch(family="megozen", vocab_size=cfg["vocab"], hidden_size=cfg["width"], layers=layers,
                   num_hidden_layers=len(layers), num_attention_heads=layers[0].mixer["heads"] if layers else 1,
                   num_key_value_heads=1, norm_eps=cfg["norm"]["eps"], block_norm="layer_norm", expert_form="glu",
@@ -535,6 +538,8 @@ class ParallelLayer(nn.Module):
     def __init__(self, a: HFArch, spec: LayerSpec, dtype):
         super().__init__()
         m = spec.mixer
+        if a.kv_cache_block and spec.type == "latent_attention":
+            raise ValueError(_NO_HEADS)
         self.input_layernorm = _block_norm(a, dtype)
         self.mlp_layernorm = _block_norm(a, dtype) if a.block_norm == "layer_norm" and spec.mlp is not None else None
         if spec.type == "attention":

@@ -172,3 +172,17 @@ def test_the_entries_refuse_rows_off_a_boundary():
         for k, v in ((at + 1, at), (at, at + 8)):
             call = cuda_infer._KV8_CALLS[name](k, v, at, at, 2, 32, 16, 16, 64, *words)
             assert getattr(cuda.lib(), name)(ctypes.c_char_p(call), ctypes.c_void_p(0)) == -2, name
+
+
+# ---- models -----------------------------------------------------------------------------------------------
+def test_latent_attention_refuses_the_cache_however_it_is_asked_for(tmp_path):
+    from easyllm_b200.models.hf_models import CausalLM, arch_from_hf_config
+    from megozen_models import CONFIGS
+    arch = arch_from_hf_config(CONFIGS["odd"])
+    CausalLM(arch).save_pretrained(str(tmp_path))
+    assert CausalLM.from_pretrained(str(tmp_path), arch_overrides={"bos_token_id": 1}).arch.bos_token_id == 1
+    with pytest.raises(ValueError, match="kv_cache_block"):
+        CausalLM.from_pretrained(str(tmp_path), arch_overrides={"kv_cache_block": 16})
+    arch.kv_cache_block = 16
+    with pytest.raises(ValueError, match="kv_cache_block"):
+        CausalLM(arch)
