@@ -98,7 +98,7 @@ def arch_from_hf_config(cfg: dict, family: Optional[str] = None) -> HFArch:
         return _pafodra_arch(cfg)
     if mt == "megozen":
         return _megozen_arch(cfg)
-    a = HFArch(family=mt, kv_cache_block=int(cfg.get("kv_cache_block", 0)))
+    a = HFArch(family=mt, kv_cache_block=int(cfg.get("kv_cache_block") or 0))
     g = cfg.get
     if mt == "qwen":
         a.vocab_size, a.hidden_size = g("vocab_size"), g("hidden_size")
@@ -194,7 +194,7 @@ def _pafodra_arch(cfg: dict) -> HFArch:
     return HFArch(family="pafodra", vocab_size=cfg["vocab"], hidden_size=cfg["width"], layers=layers,
                   num_hidden_layers=len(layers), num_attention_heads=att.get("heads", 1),
                   num_key_value_heads=att.get("kv_heads", 1), norm_eps=cfg["norm"]["eps"],
-                  embedding_scale=cfg["embedding"]["scale"], position="none", kv_cache_block=int(cfg.get("kv_cache_block", 0)),
+                  embedding_scale=cfg["embedding"]["scale"], position="none", kv_cache_block=int(cfg.get("kv_cache_block") or 0),
                   bos_token_id=cfg.get("bos_token_id"), eos_token_id=cfg.get("eos_token_id"), pad_token_id=cfg.get("pad_token_id"))
 
 

@@ -186,3 +186,12 @@ def test_latent_attention_refuses_the_cache_however_it_is_asked_for(tmp_path):
     arch.kv_cache_block = 16
     with pytest.raises(ValueError, match="kv_cache_block"):
         CausalLM(arch)
+
+
+def test_a_config_that_leaves_the_cache_empty():
+    """``null``, as tools write what is not set."""
+    from easyllm_b200.models.hf_models import arch_from_hf_config
+    from pafodra_models import CONFIGS
+    for cfg in ({"model_type": "llama"}, CONFIGS["odd"]):
+        assert arch_from_hf_config(dict(cfg, kv_cache_block=None)).kv_cache_block == 0
+        assert arch_from_hf_config(dict(cfg, kv_cache_block=8)).kv_cache_block == 8
