@@ -75,8 +75,8 @@ class KV8Rows:
     def load_prefix(self, slots, k, v):
         """Fill positions ``0 .. n`` of ``slots`` with given keys / values ``[n, kv_heads, dim]`` (prefix tuning)."""
         n, dev = k.shape[0], self.device
-        k, v = k.to(dev), v.to(dev)
-        for s in slots:
+        k, v = k.to(dev).contiguous(), v.to(dev).contiguous()         # packed heads, in whatever order the prefix has them
+        for s in slots if n else ():
             at = torch.full((n,), s * self.capacity, dtype=torch.int32, device=dev)
             iops.kv8_append(self.cache, k, v, {"kv_base": at, "kv_len": torch.arange(1, n + 1, dtype=torch.int32, device=dev), "max_seqlen": n,
                                                "cu_seqlens": torch.tensor([0, n], dtype=torch.int32, device=dev)})

@@ -195,3 +195,34 @@ def test_a_config_that_leaves_the_cache_empty():
     for cfg in ({"model_type": "llama"}, CONFIGS["odd"]):
         assert arch_from_hf_config(dict(cfg, kv_cache_block=None)).kv_cache_block == 0
         assert arch_from_hf_config(dict(cfg, kv_cache_block=8)).kv_cache_block == 8
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n,block,dtype", [(21, 16, F32), (40, 8, BF16), (1, 128, BF16), (0, 16, F32)])
+def test_a_prefix_is_held_as_the_definition_says(monkeypatch, device, n, block, dtype):
+    """Prefixes in any order of memory, into slots in any order: the rows of the definition, the other slots as they were; a step that goes
+    on inside the prefix's last block joins it."""
+    from easyllm_b200.models.hf_models.state import KV8Rows
+    from easyllm_b200.ops import cuda_infer as ci
+    dev = _device(device)
+    append = iops.kv8_append
+
+    def packed(cache, k, v, meta):                                # what the kernel takes, on the CPU too
+        ci._packed(k, "k"), ci._packed(v, "v")
+        append(cache, k, v, meta)
+    monkeypatch.setattr(iops, "kv8_append", packed)
+    slots, cap, G, d, dv = 4, 256, 3, 40, 24
+    rows = KV8Rows(slots, cap, G, d, dv, block, dev)
+    had, plain = filled(slots * cap, G, d, dv, block, dev)
+    rows.cache = had
+    k = rand(G, n, d, seed=1).to(dtype).to(dev).transpose(0, 1)   # heads first in memory
+    v = rand(n, dv, G, seed=2).to(dtype).to(dev).transpose(1, 2)
+    rows.load_prefix([3, 1], k, v)
+    more = [rand(2, G, w, seed=w).to(dtype).to(dev) for w in (d, dv)]
+    append(rows.cache, *more, step([1, 1], [n, n], [1, 3], cap, dev))
+    for s, r in ((1, 0), (3, 1)):
+        for p, x, y in zip(plain, (k, v), more):
+            p.append(s * cap, 0, x) if n else None
+            p.append(s * cap, n, y[r:r + 1])
+    for x, p in zip(iops.kv8_read(rows.cache, ints([0], dev), ints([slots * cap], dev), slots * cap, F32), plain):
+        assert torch.equal(x[0].double().cpu(), p.values(0, slots * cap))
