@@ -1438,13 +1438,6 @@ int make_tmap_bf16_2d(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_
 int make_tmap_bf16_heads(CUtensorMap* map, const void* ptr, uint64_t dim, uint64_t heads, uint64_t rows, uint64_t row_stride_bytes,
                          uint32_t box_dim, uint32_t box_rows, uint64_t head_stride_bytes);
 
-template <typename Kernel>
-static int allow_smem(Kernel kern, int smem, bool& configured) {
-  if (configured) return 0;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  configured = e == cudaSuccess;
-  return (int)e;
-}
 static int launch_attn_cached(const AttnRowsArgs& a, const AtPlan& p, const int* cu, int n_seq, long long rows, cudaStream_t stream) {
   const int rep = a.H / a.G, nh = rep < kAtHeads ? rep : kAtHeads, groups = (rep + kAtHeads - 1) / kAtHeads;
   if (p.tt == 1) cu = nullptr;
@@ -1456,15 +1449,15 @@ static int launch_attn_cached(const AttnRowsArgs& a, const AtPlan& p, const int*
   if (!rc) rc = make_tmap_bf16_heads(&tv, a.v, a.dv, a.G, rows, (uint64_t)a.ldv * 2, 64, box, 0);
   if (rc) return rc;
   if (!p.few) {
-    static bool tile = false;
-    if ((rc = allow_smem(attn_tile_kernel, kAtSmem, tile)) != 0) return rc;
+    static SmemLimit limit;
+    if ((rc = allow_smem(attn_tile_kernel, kAtSmem, limit)) != 0) return rc;
     launch_chained(attn_tile_kernel, grid, kAtTileThreads, kAtSmem, stream, tk, tv, a, cu, p.tiles, p.tt);
   } else {
     const bool full = a.d == 128 && a.dv == 128, small = p.tt * nh <= 8;
 #define ELL_FEW(NB_, FULL_)                                                                                                   \
   if (small == (NB_ == 1) && full == FULL_) {                                                                                 \
-    static bool ready = false;                                                                                                \
-    if ((rc = allow_smem(attn_few_kernel<NB_, FULL_>, kAfSmem, ready)) != 0) return rc;                                       \
+    static SmemLimit limit;                                                                                                   \
+    if ((rc = allow_smem(attn_few_kernel<NB_, FULL_>, kAfSmem, limit)) != 0) return rc;                                       \
     launch_chained(attn_few_kernel<NB_, FULL_>, grid, kAtThreads, kAfSmem, stream, tk, tv, a, cu, p.tiles, p.tt);              \
   }
     ELL_FEW(1, true)
@@ -1495,12 +1488,8 @@ static int launch_attn_latent(const AttnRowsArgs& a, long long rows, cudaStream_
   const int rc = make_tmap_bf16_2d(&tk, a.k, (uint64_t)a.d, (uint64_t)rows, (uint64_t)a.ldk * 2, 64, kAlKeys);
   if (rc) return rc;
   const int bytes = al_bytes(a.d, MT);
-  static int configured = 0;
-  if (bytes > configured) {
-    cudaError_t e = cudaFuncSetAttribute(attn_latent_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return (int)e;
-    configured = bytes;
-  }
+  static SmemLimit limit;
+  if (const int e = allow_smem(attn_latent_kernel<MT>, bytes, limit)) return e;
   launch_chained(attn_latent_kernel<MT>, dim3(a.n, (a.H + 16 * MT - 1) / (16 * MT), a.splits), kAlWarps * 32, bytes, stream, tk, a);
   if (a.splits > 1) launch_chained(attn_rows_merge_kernel<__nv_bfloat16>, dim3(a.n, a.H), kArThreads, 0, stream, a);
   return launch_status();
@@ -1530,12 +1519,8 @@ template <typename T, int KT, int REP, bool VEC>
 static int launch_attn_rows_kt(const AttnRowsArgs& a, dim3 grid, cudaStream_t stream) {
   const int bytes = ar_layout(a.d, a.dv, sizeof(T), KT, REP).bytes;
   auto kern = attn_rows_kernel<T, KT, REP, VEC>;
-  static int configured = 0;
-  if (bytes > configured) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return (int)e;
-    configured = bytes;
-  }
+  static SmemLimit limit;
+  if (const int e = allow_smem(kern, bytes, limit)) return e;
   launch_chained(kern, grid, kArThreads, bytes, stream, a);
   if (a.splits > 1) launch_chained(attn_rows_merge_kernel<T>, dim3(a.n, a.H), kArThreads, 0, stream, a);
   return launch_status();

@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "smem_limit.h"
+
 #define ELL_API extern "C" __attribute__((visibility("default")))
 
 namespace ell {

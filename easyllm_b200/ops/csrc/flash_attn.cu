@@ -557,12 +557,8 @@ static int launch_flash_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const 
   const int rc = make_tmap_bf16_heads(&to, fa.out, fa.dv, fa.Hq, fa.T, (uint64_t)fa.Hq * fa.dv * 2, 64, 32);
   if (rc) return rc;
   auto kern = flash_fwd_kernel<KN, NC>;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FaCfg<KN, NC>::kSmemBytes);
-    if (e != cudaSuccess) return (int)e;
-    configured = true;
-  }
+  static SmemLimit limit;
+  if (const int e = allow_smem(kern, FaCfg<KN, NC>::kSmemBytes, limit)) return e;
   const long long grid = (long long)((fa.T + 2 * kFaM - 1) / (2 * kFaM)) * fa.Hq;
   if (grid > 0x7fffffff) return -2;
   FaArgs args = fa;

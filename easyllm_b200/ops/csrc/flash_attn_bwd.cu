@@ -839,13 +839,9 @@ ELL_API int ell_flash_attn_bwd(const void* q, const void* k, const void* v, cons
     if (!rc) rc = make_tmap_bf16_heads(&tdv, dv, kFbD, Hk, T, (uint64_t)dkv_stride * 2, 64, 32);
   }
   if (rc) return rc;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(flash_bwd_kv_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFbKvSmem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(flash_bwd_q_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFbQSmem);
-    if (e != cudaSuccess) return (int)e;
-    configured = true;
-  }
+  static SmemLimit kv_limit, q_limit;
+  if (const int e = allow_smem(flash_bwd_kv_kernel, kFbKvSmem, kv_limit)) return e;
+  if (const int e = allow_smem(flash_bwd_q_kernel, kFbQSmem, q_limit)) return e;
   if (nsplit > 1) {
     cudaError_t e = cudaMemsetAsync(dkv_acc, 0, (size_t)2 * T * Wk * sizeof(float), stream);
     if (e != cudaSuccess) return (int)e;

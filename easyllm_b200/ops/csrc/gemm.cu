@@ -617,12 +617,8 @@ static int launch_gemm(const CUtensorMap& tA, const CUtensorMap& tB, const CUten
                        const __nv_bfloat16* bias, int M, int N, int K, int ldc, int* err, int max_ctas,
                        cudaStream_t stream, const CUtensorMap* tA2 = nullptr) {
   auto kern = gemm_bf16_kernel<BN, A_MN, B_MN, OUT, HAS_BIAS, FUSE>;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmCfg<BN>::kSmemBytes);
-    if (e != cudaSuccess) return (int)e;
-    configured = true;
-  }
+  static SmemLimit limit;
+  if (const int e = allow_smem(kern, GemmCfg<BN>::kSmemBytes, limit)) return e;
   const int tiles = ((M + kBM - 1) / kBM) * ((N + BN - 1) / BN);
   int grid = (FUSE != kFuseNone || tiles >= max_ctas) ? max_ctas : tiles;   // fused launches keep a fixed grid
   if ((FUSE == kFuseNone || FUSE == kFuseGroup) && M <= kChainedRows)

@@ -990,12 +990,8 @@ static int launch(const CUtensorMap& tA, const CUtensorMap& tB, const CUtensorMa
                   const CUtensorMap& tX, const FuseArgs& fuse, const __nv_bfloat16* bias, int M, int N, int K, int* err,
                   cudaStream_t stream, const FuseArgs* push = nullptr) {
   auto kern = gemm_pair_kernel<A_MN, B_MN, OUT, HAS_BIAS, FUSE>;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-    if (e != cudaSuccess) return (int)e;
-    configured = true;
-  }
+  static SmemLimit limit;
+  if (const int e = allow_smem(kern, kSmemBytes, limit)) return e;
   const int resident = max_clusters(reinterpret_cast<const void*>(kern));
   if (resident <= 0) return -20;                 // the device cannot co-schedule a pair with this much shared memory
   const int tiles = ((M + kTileM - 1) / kTileM) * ((N + kTileN - 1) / kTileN);
@@ -1031,7 +1027,8 @@ static int launch(const CUtensorMap& tA, const CUtensorMap& tB, const CUtensorMa
 
 static int resident_clusters() {
   auto kern = gemm_pair_kernel<false, false, kOutBf16, false, kFuseNone>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) != cudaSuccess) {
+  static SmemLimit limit;
+  if (allow_smem(kern, kSmemBytes, limit) != 0) {
     cudaGetLastError();
     return -1;
   }

@@ -409,11 +409,11 @@ static int launch_thin(const CUtensorMap& tw, const CUtensorMap& tx, ThinArgs a,
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
+  static SmemLimit limit;
+  if (const int e = allow_smem(kern, ThinCfg<BN>::kSmemBytes, limit)) return e;
   // clusters of 1, 2, 4, 8 CTAs that are resident together: a cluster lies within one GPC, so fewer than SMs / size
   static int clusters[4] = {0, 0, 0, 0};
   if (clusters[0] == 0) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ThinCfg<BN>::kSmemBytes);
-    if (e != cudaSuccess) return (int)e;
     int found[4] = {0, 0, 0, 0}, dev = 0;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&found[0], cudaDevAttrMultiProcessorCount, dev);

@@ -1089,12 +1089,8 @@ int make_tmap_bytes_heads(CUtensorMap* map, const void* ptr, uint64_t dim, uint6
 
 template <typename T, int NB>
 static int launch_attn_kv8(const Kv8Attn& a, const K8Plan& p, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t stream) {
-  static bool ready = false;
-  if (!ready) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, k8_smem<NB>());
-    if (e != cudaSuccess) return (int)e;
-    ready = true;
-  }
+  static SmemLimit limit;
+  if (const int e = allow_smem(attn_kv8_kernel<T, NB>, k8_smem<NB>(), limit)) return e;
   launch_chained(attn_kv8_kernel<T, NB>, p.ctas, kK8Threads, k8_smem<NB>(), stream, tk, tv, a);
   if (p.cut) launch_chained(attn_kv8_join_kernel<T, 8 * NB>, p.ctas, kK8JoinThreads, 0, stream, a);
   return launch_status();

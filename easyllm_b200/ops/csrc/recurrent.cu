@@ -356,12 +356,8 @@ template <int MODE, typename T, int DP>
 int launch_scan(const ScanArgs& a, int n_seq, int vec, cudaStream_t stream) {
   constexpr int bytes = scan_smem_bytes<T, DP>();
   auto kern = scan_kernel<MODE, T, DP>;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return (int)e;
-    configured = true;
-  }
+  static SmemLimit limit;
+  if (const int e = allow_smem(kern, bytes, limit)) return e;
   dim3 grid((a.dv + kScanCols - 1) / kScanCols, a.H, n_seq);
   // Not chained: CTAs that come in while the kernel before ends are packed where there is room first, and with two CTAs on an SM
   // a scan of 4096 tokens took 1.5 times as long.

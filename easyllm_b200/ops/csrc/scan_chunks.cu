@@ -704,12 +704,8 @@ template <int MODE, typename T, int DP>
 static int launch_chunks(ChunkArgs a, const ChunkPlan& p, int n_seq, cudaStream_t stream) {
   auto scan = chunk_scan_kernel<MODE, T, DP>;
   constexpr int bytes = ScanSmem<MODE, DP>::kBytes;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return (int)e;
-    configured = true;
-  }
+  static SmemLimit limit;
+  if (const int e = allow_smem(scan, bytes, limit)) return e;
   a.per_seq = p.by_tokens ? 0 : p.round;
   for (int c0 = 0; c0 < p.chunks; c0 += p.round) {
     a.c0 = c0;

@@ -127,3 +127,57 @@ def test_operands_updated_in_place_keep_their_order(rows):
         torch.cuda.synchronize()
         cu.check_err_flag()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_shared_memory_is_asked_for_on_every_device(tmp_path):
+    """The limit of a kernel's dynamic shared memory is that of one device.  No launcher sets it by itself; what they use asks each device
+    once for each kernel, and again where a launch needs more."""
+    import shutil
+    import subprocess
+    for path in sorted(glob.glob(os.path.join(CSRC, "*.c*"))):
+        assert "cudaFuncSetAttribute" not in open(path).read(), path
+    inc = "/usr/local/cuda/include"
+    if shutil.which("g++") is None or not os.path.exists(inc):
+        pytest.skip("no compiler")
+    program = r'''
+#include "smem_limit.h"
+#include <cstdio>
+static int device = 0, fail = 0;
+extern "C" cudaError_t cudaGetDevice(int* d) { *d = device; return cudaSuccess; }
+extern "C" cudaError_t cudaFuncSetAttribute(const void* f, cudaFuncAttribute, int bytes) {
+  std::printf("%d:%c:%d ", device, f == (const void*)1 ? 'a' : 'b', bytes);
+  return fail ? cudaErrorInvalidValue : cudaSuccess;
+}
+static ell::SmemLimit a, b;
+static void ask(int dev, long kernel, int bytes) {
+  device = dev;
+  std::printf("%d ", ell::allow_smem_of((const void*)kernel, bytes, kernel == 1 ? a : b));
+}
+int main() {
+  ask(0, 1, 100000), ask(0, 1, 100000), ask(1, 1, 100000), ask(1, 1, 90000), ask(0, 2, 60000), ask(1, 1, 120000), ask(0, 1, 100000);
+  fail = 1, ask(2, 1, 5), fail = 0, ask(2, 1, 5), ask(100, 1, 7), ask(100, 1, 7);
+}
+'''
+    src, exe = tmp_path / "limit.cpp", tmp_path / "limit"
+    src.write_text(program)
+    subprocess.run(["g++", "-std=c++17", "-I", CSRC, "-I", inc, str(src), "-o", str(exe), "-pthread"], check=True, capture_output=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
+    assert out.split() == ("0:a:100000 0 0 1:a:100000 0 0 0:b:60000 0 1:a:120000 0 0 2:a:5 1 2:a:5 0 100:a:7 0 100:a:7 0").split()
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_a_kernel_runs_on_a_second_device():
+    """The same call on one device and then on another, with the first one current."""
+    from easyllm_b200.ops import cuda
+    from easyllm_b200.ops import infer as iops
+    cuda.lib()
+    out = []
+    for dev in ("cuda:0", "cuda:1"):
+        cache = iops.kv8_empty(64, 2, 32, 32, 16, dev)
+        x = torch.randn(5, 2, 32, generator=torch.Generator().manual_seed(1)).to(dev)
+        base, length = torch.zeros(5, dtype=torch.int32, device=dev), torch.arange(1, 6, dtype=torch.int32, device=dev)
+        cu = torch.tensor([0, 5], dtype=torch.int32, device=dev)
+        iops.kv8_append(cache, x, x, {"kv_base": base, "kv_len": length, "cu_seqlens": cu, "max_seqlen": 5})
+        out.append(iops.attention_kv8(x.repeat(1, 2, 1), cache, base, length, 5, 0.2).cpu())
+    assert torch.equal(*out)
