@@ -1149,10 +1149,11 @@ static bool k8_cache(const Kv8Args& a, Kv8Cache& c) {
 ELL_API int ell_kv8_append(const Kv8AppendCall* call, cudaStream_t stream) {
   const Kv8AppendCall& x = *call;
   Kv8Cache c;
-  if (x.n <= 0 || x.n_seq <= 0 || x.max_new <= 0) return 0;
+  if (x.n <= 0 || x.n_seq <= 0) return 0;
   if (!k8_cache(x.c, c) || x.n > 0x7fffffff) return -2;
   const int esz = x.is_bf16 ? 2 : 4;
-  const long long blocks = (x.max_new + 2 * x.c.block - 2) / x.c.block, ctas = blocks * ((2 * c.G + 7) / 8);
+  // a bound below 1 is that of sequences without rows: one that has some all the same is found out by the first block's CTAs
+  const long long blocks = (std::max(x.max_new, 1ll) + 2 * x.c.block - 2) / x.c.block, ctas = blocks * ((2 * c.G + 7) / 8);
   if (ctas > 0x7fffffff || x.n_seq > 65535) return -2;
   const bool vec = c.d % 8 == 0 && c.dv % 8 == 0 && x.ldk * esz % 16 == 0 && x.ldv * esz % 16 == 0 && aligned_to(x.k, 16) && aligned_to(x.v, 16);
 #define ELL_APPEND(T, V)                                                                                                                \

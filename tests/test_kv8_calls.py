@@ -174,6 +174,36 @@ def test_the_entries_refuse_rows_off_a_boundary():
             assert getattr(cuda.lib(), name)(ctypes.c_char_p(call), ctypes.c_void_p(0)) == -2, name
 
 
+# ---- bounds that do not hold --------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("bound", [0, -3])
+@pytest.mark.parametrize("n,start", [(40, 0), (17, 16), (30, 9)])
+def test_rows_beyond_a_bound_of_none_are_reported(bound, n, start):
+    """``max_seqlen`` below 1 with a sequence that brings more rows than a block takes: the error word is set, as with any other bound
+    that does not hold, and what was written before the bound is a whole block."""
+    from easyllm_b200.ops import cuda
+    dev = _device("cuda")
+    cache, plain = filled(128, 2, 32, 32, 16, dev)
+    x = rand(n, 2, 32, seed=1).to(dev)
+    iops.kv8_append(cache, x, x, dict(step([n], [start], [0], 128, dev), max_seqlen=bound))
+    with pytest.raises(cuda.KernelError, match="51"):
+        cuda.check_err_flag()
+    for p in plain:
+        p.append(0, start, x[:16 - start % 16])
+    for got, p in zip(iops.kv8_read(cache, ints([0], dev), ints([128], dev), 128, F32), plain):
+        assert torch.equal(got[0].double().cpu(), p.values(0, 128))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_bound_of_none_with_no_rows(device):
+    dev = _device(device)
+    cache, plain = filled(128, 2, 32, 32, 16, dev)
+    x = rand(3, 2, 32, seed=1).to(dev)
+    iops.kv8_append(cache, x, x, {"kv_base": ints([0] * 3, dev), "kv_len": ints([5, 6, 7], dev), "cu_seqlens": ints([0, 0, 0], dev), "max_seqlen": 0})
+    for got, p in zip(iops.kv8_read(cache, ints([0], dev), ints([128], dev), 128, F32), plain):
+        assert torch.equal(got[0].double().cpu(), p.values(0, 128))
+
+
 # ---- models -----------------------------------------------------------------------------------------------
 def test_latent_attention_refuses_the_cache_however_it_is_asked_for(tmp_path):
     from easyllm_b200.models.hf_models import CausalLM, arch_from_hf_config
