@@ -350,6 +350,7 @@ def kv8_read(base, length, words, max_len, dtype):
 # 128 70 | 74, 256 123 | 100; 1 of 30000, 64/8, 128 108 | 91, 256 195 | 126; 8 of 2000, 32/8, 256 58 | 67, 512 102 | 107, 1024 192 | 120;
 # 2 of 400, 32/8, 256 21 | 27, 512 29 | 27.
 KV8_READ_ROWS, KV8_READ_LONG, KV8_READ_BYTES = 512, (256, 4096), 1 << 30
+KV8_READ_SEQUENCES = 65535          # the reading kernel's grid
 KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 1024, 296, 4232
 
 
@@ -371,7 +372,7 @@ def attention_kv8(q, words, base, length, max_len, scale, sink, alibi_slopes, wi
     n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, max_q)
     rows = max_q * (H // G)
     if max_q > 1 and (rows >= KV8_READ_ROWS or (rows >= KV8_READ_LONG[0] and max_len >= KV8_READ_LONG[1])) and q.dtype is torch.bfloat16 and \
-            not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4) and 2 * n_seq * max_len * G * (d + dv) <= KV8_READ_BYTES:
+            n_seq <= KV8_READ_SEQUENCES and not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4) and 2 * n_seq * max_len * G * (d + dv) <= KV8_READ_BYTES:
         return _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
     out = q.new_empty((T, H, dv))
     # room for what shares cut: a call has no more CTAs than are resident, or a CTA for each key head and 16 of its query heads

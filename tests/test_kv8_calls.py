@@ -73,6 +73,27 @@ def test_single_tokens_stay_on_the_bytes_whatever_their_heads(monkeypatch):
             assert way(monkeypatch, 3, H, cache, max_len, ints([0, 2]), 2) == ("back" if 2 * H >= 512 else "bytes")
 
 
+def test_more_sequences_than_are_read_back_stay_on_the_bytes(monkeypatch):
+    cache = iops.kv8_empty(64, 1, 16, 16, 16)
+    for n, want in ((65535, "back"), (65536, "bytes")):
+        cu = torch.arange(n + 1, dtype=torch.int32)
+        assert way(monkeypatch, n, 16, cache, 64, cu, 32) == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("device", ["cuda"])
+def test_attention_of_more_sequences_than_are_read_back(device):
+    """65536 sequences, of 32 tokens the first and the last, the others of none."""
+    dev = _device(device)
+    cache, plain = filled(128, 1, 16, 16, 16, dev)
+    q = rand(64, 16, 16, seed=1).to(BF16).to(dev)
+    base, length = ints([0] * 32 + [64] * 32, dev), ints(list(range(20, 52)) + list(range(1, 33)), dev)
+    cu = ints([0] + [32] * 65535 + [64], dev)
+    got = iops.attention_kv8(q, cache, base, length, 64, 0.3, cu_seqlens=cu, max_q=32)
+    for r, (b, n) in enumerate(zip(base.tolist(), length.tolist())):
+        near(got[r], *plain_attention(q[r], *(p.values(b, n) for p in plain), 0.3))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("device", ["cuda"])
 @pytest.mark.parametrize("H,longest,block", [(512, 90, 16), (256, 4200, 64), (512, 4200, 16), (258, 4200, 16)])
