@@ -180,12 +180,12 @@ class DecodeState:
 
 class DecodeGraph:
     """The one-token step of fixed slots as a CUDA graph: embedding, layers, logits and the advance of the positions,
-    replayed with new token ids.  The cache must not move while the graph is in use: its capacity is checked, and the
-    caller captures anew when the state has grown.  Capturing executes nothing, so no state is touched; run at least one
+    replayed with new token ids.  The cache must not move while the graph is in use: that it has not grown, in positions or
+    slots, is checked, and the caller captures anew when it has.  Capturing executes nothing, so no state is touched; run at least one
     eager step before (it initialises the kernels)."""
 
     def __init__(self, model, state, slots):
-        self.state, self.slots, self.capacity = state, list(slots), state.capacity
+        self.state, self.slots, self.capacity, self.state_slots = state, list(slots), state.capacity, state.slots
         self.meta = state.step_meta(slots, [1] * len(slots), advance=False)
         # host-side bounds that hold for every replay
         self.meta.update(max_position=state.capacity, kv_bound=state.capacity, fresh=False, one_token=True)
@@ -202,7 +202,7 @@ class DecodeGraph:
     def step(self, tokens):
         """fp32 logits ``[n, vocab]`` after ``tokens [n]`` (a buffer the next step overwrites)."""
         st = self.state
-        if st.capacity != self.capacity or any(st.lengths[s] >= self.capacity for s in self.slots):
+        if (st.capacity, st.slots) != (self.capacity, self.state_slots) or any(st.lengths[s] >= self.capacity for s in self.slots):
             raise RuntimeError("the cache moved or is full: capture the decode step again")
         self.ids.copy_(tokens)
         self.graph.replay()

@@ -277,3 +277,40 @@ def test_a_prefix_is_held_as_the_definition_says(monkeypatch, device, n, block, 
             p.append(s * cap, n, y[r:r + 1])
     for x, p in zip(iops.kv8_read(rows.cache, ints([0], dev), ints([slots * cap], dev), slots * cap, F32), plain):
         assert torch.equal(x[0].double().cpu(), p.values(0, slots * cap))
+
+
+@pytest.mark.gpu
+def test_a_captured_step_is_not_replayed_once_the_state_has_grown():
+    """A state without a free slot grows by a new sequence: its caches are elsewhere then, whatever their kind."""
+    from easyllm_b200.models.hf_models.state import DecodeGraph
+    from test_kv8 import _model
+    dev = _device("cuda")
+    for block in (0, 16):
+        m = _model("llama", dev, BF16, kv_cache_block=block)
+        state = m.new_state(1, 40)
+        slot = state.open()
+        m.step(state, [slot], [list(range(20))])
+        ids = torch.tensor([7], device=dev)
+        m.logits(m.step(state, [slot], ids)[0])
+        graph = DecodeGraph(m, state, [slot])
+        graph.step(ids)
+        state.open()
+        with pytest.raises(RuntimeError, match="capture"):
+            graph.step(ids)
+
+
+def test_growth_in_slots_and_in_positions_ends_a_graph():
+    from types import SimpleNamespace
+    from easyllm_b200.models.hf_models.state import DecodeGraph
+    replays = []
+    graph = DecodeGraph.__new__(DecodeGraph)
+    graph.slots, graph.capacity, graph.state_slots, graph.ids, graph.logits = [1], 256, 2, torch.zeros(1, dtype=torch.long), None
+    graph.graph = SimpleNamespace(replay=lambda: replays.append(1))
+    for capacity, lengths, fine in ((256, [3, 9], True), (256, [3, 9, 0, 0], False), (512, [3, 9], False), (256, [3, 256], False)):
+        graph.state = SimpleNamespace(capacity=capacity, slots=len(lengths), lengths=lengths)
+        if fine:
+            graph.step(torch.ones(1, dtype=torch.long))
+        else:
+            with pytest.raises(RuntimeError, match="capture"):
+                graph.step(torch.ones(1, dtype=torch.long))
+    assert len(replays) == 1
