@@ -314,3 +314,168 @@ def test_growth_in_slots_and_in_positions_ends_a_graph():
             with pytest.raises(RuntimeError, match="capture"):
                 graph.step(torch.ones(1, dtype=torch.long))
     assert len(replays) == 1
+
+
+def _hybrid(name, dev, dtype, **kw):
+    from easyllm_b200.models.hf_models import CausalLM, arch_from_hf_config
+    from pafodra_models import CONFIGS
+    torch.manual_seed(0)
+    m = CausalLM(arch_from_hf_config(dict(CONFIGS[name], **kw)), dtype)
+    for n, p in m.named_parameters():                             # states that neither vanish nor blow up, sinks that count
+        if n.endswith("sink"):
+            p.data.normal_(1.0)
+    return m.to(dev).eval()
+
+
+class Watch:
+    """Looks over the calls that a model makes of the cache: keeps, for each layer and sequence, what a cache should hold by the test's own
+    count of positions, and holds every answer of the attention against it."""
+
+    def __init__(self, monkeypatch, block):
+        self.block, self.held, self.rows, self.appended, self.attended, self.calls = block, {}, [], 0, 0, []
+        self.append, self.attend = iops.kv8_append, iops.attention_kv8
+        monkeypatch.setattr(iops, "kv8_append", self.on_append)
+        monkeypatch.setattr(iops, "attention_kv8", self.on_attend)
+
+    def begin(self, rows):
+        """``rows``: (sequence, positions it has, tokens) of the step, in the order of its rows."""
+        self.rows, self.layer = rows, -1
+
+    def on_append(self, cache, k, v, meta):
+        from test_kv8 import Plain
+        self.layer += 1
+        self.appended += 1
+        self.calls.append((self.layer, k.clone(), v.clone()))
+        self.append(cache, k, v, meta)
+        r = 0
+        for seq, start, n in self.rows:
+            held = self.held.setdefault((self.layer, seq), [Plain(384, x.shape[1], x.shape[2], self.block) for x in (k, v)])
+            for p, x in zip(held, (k, v)):
+                p.append(0, start, x[r:r + n])
+            r += n
+        assert r == k.shape[0]
+
+    def on_attend(self, q, cache, base, length, max_len, scale, sink=None, slopes=None, **kw):
+        got = self.attend(q, cache, base, length, max_len, scale, sink, slopes, **kw)
+        self.attended += 1
+        r = 0
+        for seq, start, n in self.rows:
+            for j in range(n):
+                if j in (0, 1, n // 2, n - 1):                    # of a prompt some rows
+                    keys, values = (p.values(0, start + j + 1) for p in self.held[self.layer, seq])
+                    near(got[r + j], *plain_attention(q[r + j], keys, values, scale, sink, slopes))
+            r += n
+        return got
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["llama", "alibi", "qwen", "aligned", "odd"])
+def test_every_layer_attends_to_what_its_cache_should_hold(monkeypatch, device, dtype, kind):
+    """Ragged prompts, a state that grows in slots and in positions, decoding, a prompt beside decoding sequences, a slot used again: in
+    every layer that attends, hybrid models' too, each answer is that of the rows which a cache kept by the test's own count would hold."""
+    from test_kv8 import _model
+    dev = _device(device)
+    hybrid = kind in ("aligned", "odd")
+    m = _hybrid(kind, dev, dtype, kv_cache_block=8) if hybrid else _model(kind, dev, dtype, kv_cache_block=8)
+    attending = sum(l.type == "attention" for l in m.arch.layers) if hybrid else 2
+    watch = Watch(monkeypatch, 8)
+    state = m.new_state(1, 10)
+    ids = torch.randint(0, 80, (400,), generator=torch.Generator().manual_seed(1))
+    lengths, slots, at, steps = {}, {}, 0, 0
+    for step_ in ([("a", 250), ("b", 9)], [("a", 1), ("b", 1)], [("b", 1), ("a", 1)], [("a", 1), ("c", 13), ("b", 2)], [("a", 3)],
+                  [("c", 1), ("b", 1), ("a", 1)], ["close b"], [("a", 1), ("d", 21)], [("d", 1), ("c", 1), ("a", 1)]):
+        if step_ == ["close b"]:
+            state.close(slots["b"])
+            continue
+        for s, _ in step_:
+            if s not in slots:
+                slots[s], lengths[s] = state.open(), 0
+        watch.begin([(s, lengths[s], n) for s, n in step_])
+        m.step(state, [slots[s] for s, _ in step_], [ids[at + i:at + i + n] for i, (_, n) in enumerate(step_)])
+        for s, n in step_:
+            lengths[s] += n
+        at, steps = at + 7, steps + 1
+        assert watch.layer == attending - 1
+    assert slots["d"] == slots["b"] and state.capacity > 256 and state.slots > 2
+    # a step of prompts alone may attend to its own keys, every other one looks into the cache
+    assert watch.appended == steps * attending and watch.attended >= (steps - 1) * attending
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", ["llama", "qwen", "aligned"])
+def test_what_a_layer_writes_is_what_it_would_write_in_full(monkeypatch, device, kind):
+    """The first attending layer's keys and values of a prompt, as the model without the 8-bit cache hands them to its own."""
+    from test_kv8 import _model
+    dev = _device(device)
+    wrote = {}
+    for block in (8, 0):
+        m = _hybrid(kind, dev, F32, kv_cache_block=block) if kind == "aligned" else _model(kind, dev, F32, kv_cache_block=block)
+        with monkeypatch.context() as patch:
+            patch.setattr(iops, "kv8_append", lambda cache, k, v, meta: wrote.setdefault(8, (k.clone(), v.clone())))
+            patch.setattr(iops, "attention_kv8", lambda q, cache, *a, **kw: q.new_zeros(*q.shape[:2], cache.vdim))
+            patch.setattr(iops, "kv_append", lambda kc, vc, k, v, meta: wrote.setdefault(0, (k.clone(), v.clone())))
+            state = m.new_state(2, 40)
+            m.step(state, [state.open(), state.open()], [list(range(30)), list(range(5, 16))])
+    assert all(torch.equal(a, b) for a, b in zip(wrote[8], wrote[0]))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_hybrid_model_generates_from_8_bits(device):
+    """Rows of unequal length give the tokens that each gives alone; on a GPU through the captured step as without it."""
+    dev = _device(device)
+    m = _hybrid("aligned", dev, F32, kv_cache_block=16)
+    ids = torch.randint(0, 264, (3, 12), generator=torch.Generator().manual_seed(2)).to(dev)
+    mask = torch.ones_like(ids)
+    mask[1, :5] = 0
+    out = m.generate(ids, attention_mask=mask, max_new_tokens=9)
+    assert torch.equal(out[1, 12:], m.generate(ids[1:2, 5:], max_new_tokens=9)[0, 7:])
+    assert torch.equal(out, m.generate(ids, attention_mask=mask, max_new_tokens=9, cuda_graph=False))
+
+
+# ---- memory that nobody wrote ---------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,kind", [(None, None), (90, None), (None, "sink"), (None, "alibi")])
+@pytest.mark.parametrize("H,G,d,dv", [(8, 2, 128, 128), (16, 1, 48, 64)])
+def test_rows_read_back_do_not_depend_on_what_lay_behind_them(monkeypatch, H, G, d, dv, window, kind):
+    """Long continued prompts of unequal length, a sequence without rows, one whose rows see nothing, rows behind the last border: the bits
+    are the same when all memory that the call allocates held NaN before."""
+    from easyllm_b200.ops import cuda_infer as ci
+    dev = _device("cuda")
+    cap, total, new = 1024, [700, 65, 64, 330], [150, 1, 64, 129]
+    cache, plain = filled(4 * cap, G, d, dv, 16, dev)
+    meta = step(new, [t - c for t, c in zip(total, new)], [3, 0, 2, 1], cap, dev)
+    T, dead = sum(new), 7
+    base = torch.cat((meta["kv_base"], ints([5] * dead, dev)))
+    length = torch.cat((meta["kv_len"], ints([0, 0, 0, 900, 901, 902, 903], dev)))
+    cu = ints(meta["cu_seqlens"].tolist()[:2] + meta["cu_seqlens"].tolist()[1:] + [T + 3], dev)         # the second sequence is empty, the last sees nothing
+    q = rand(T + dead, H, d, seed=1).to(BF16).to(dev)
+    sink = rand(H, seed=4).to(dev) if kind == "sink" else None
+    slopes = torch.tensor([2.0 ** (-8.0 * (h + 1) / H) for h in range(H)]).to(dev) if kind == "alibi" else None
+    taken = []
+    back = ci._attention_read_back
+    monkeypatch.setattr(ci, "_attention_read_back", lambda *a: (taken.append(1), back(*a))[1])
+
+    def call():
+        return iops.attention_kv8(q, cache, base, length, 720, 0.1, sink, slopes, window, cu, 160)
+    want = call()
+    empty, poisoned = torch.empty, []
+
+    def held_nan(*a, **kw):
+        t = empty(*a, **kw)
+        if t.is_cuda and t.is_floating_point():
+            t.fill_(float("nan"))
+            poisoned.append(t.numel())
+        return t
+    with monkeypatch.context() as patch:
+        patch.setattr(torch, "empty", held_nan)
+        got = call()
+    assert len(taken) == 2 and len(poisoned) >= 3 and torch.equal(got, want) and not bool(got[T:].any())
+    assert bool(got.isfinite().all())
+    r = 0
+    for t, n, s in zip(total, new, (3, 0, 2, 1)):
+        for j in sorted({0, n // 2, n - 1}):
+            end = t - n + j + 1
+            low = max(0, end - window) if window else 0
+            near(got[r + j], *plain_attention(q[r + j], *(p.values(s * cap + low, end - low) for p in plain), 0.1, sink, slopes))
+        r += n
