@@ -373,7 +373,7 @@ struct Kv8Attn {
   float* part;                    // when shares are cut: two slots a CTA, then the CTAs' K8Cut
   const int *base, *len, *cu;
   const float *sink, *slopes;
-  int n, H, ldq, n_seq, tiles, tt, cut, window;
+  int n, H, ldq, n_seq, tiles, tt, cut, window, max_len;
   float scale;                    // of the scores, times log2 e 2^-21
   int* err;
 };
@@ -401,10 +401,9 @@ struct K8Tile {
     len0 = a.len[r0];
     len1 = a.len[r1 - 1];
     base = a.base[r0];
-    if (len1 > 0 && !k8_inside(a.c, base, len1)) {
-      atomicCAS(a.err, 0, kK8Place);
-      len1 = 0;
-    }
+    const bool in = len1 <= 0 || k8_inside(a.c, base, len1);
+    if (!in || len1 > a.max_len) atomicCAS(a.err, 0, kK8Place);        // a longer sequence than was said is answered all the same
+    if (!in) len1 = 0;
     len1 = max(len1, 0);
     len0 = min(max(len0, 0), len1);
     low = max(0, len0 - a.window) & ~(kK8Keys - 1);
@@ -1209,6 +1208,7 @@ ELL_API int ell_attn_kv8(const Kv8AttnCall* call, cudaStream_t stream) {
   if (p.cut && (x.part == nullptr || !aligned_to(x.part, 16) || (size_t)x.part_floats < k8_part_floats(p))) return -2;
   a.q = x.q, a.out = x.out, a.part = x.part, a.base = x.base, a.len = x.len, a.cu = x.cu, a.sink = x.sink, a.slopes = x.slopes;
   a.n = (int)x.n, a.H = (int)x.H, a.ldq = (int)x.ldq, a.n_seq = n_seq, a.tiles = p.tiles, a.tt = p.tt, a.cut = p.cut;
+  a.max_len = (int)std::max(x.max_len, 0ll);
   a.window = x.window > 0 ? (int)std::min(x.window, 0x3fffffffll) : 0x3fffffff;
   a.scale = (float)(x.scale * 1.4426950408889634 / 2097152);
   a.err = x.err;

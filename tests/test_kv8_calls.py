@@ -215,6 +215,28 @@ def test_rows_beyond_a_bound_of_none_are_reported(bound, n, start):
         assert torch.equal(got[0].double().cpu(), p.values(0, 128))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("max_len,total,new", [(10, 40, 1), (0, 1, 1), (-5, 7, 3), (64, 65, 1), (1100, 1300, 2)])
+def test_lengths_beyond_their_bound_are_reported(dtype, max_len, total, new):
+    """By the attention on the cache's bytes as by that on rows read back; there the answers are those of the true lengths."""
+    from easyllm_b200.ops import cuda
+    dev = _device("cuda")
+    cache, plain = filled(1408, 2, 32, 32, 16, dev)
+    meta = step([new], [total - new], [0], 1408, dev)
+    q = rand(new, 4, 32, seed=3).to(dtype).to(dev)
+    kw = dict(cu_seqlens=meta["cu_seqlens"], max_q=new) if new > 1 else {}
+    for bound, fine in ((total, True), (max_len, False)):
+        got = iops.attention_kv8(q, cache, meta["kv_base"], meta["kv_len"], bound, 0.2, **kw)
+        if fine:
+            cuda.check_err_flag()
+        else:
+            with pytest.raises(cuda.KernelError, match="51"):
+                cuda.check_err_flag()
+        for r in range(new):
+            near(got[r], *plain_attention(q[r], *(p.values(0, total - new + 1 + r) for p in plain), 0.2))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_a_bound_of_none_with_no_rows(device):
     dev = _device(device)
