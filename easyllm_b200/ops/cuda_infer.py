@@ -344,14 +344,27 @@ def kv8_read(base, length, words, max_len, dtype):
 
 
 # Continued prompts with many rows (tokens times query heads of a key head): the cache's rows are written out in bf16 once and the tcgen05
-# kernel attends to those, while that takes no more memory than this.  That kernel goes by the borders of sequences of several tokens; single
-# ones, however many heads they have, stay on the cache's bytes.  Us of the integer products on the cache | of rows read back
-# (sequences, keys, query and key heads, rows): 1 of 4096, 32/8, 128 rows 29 | 31, 256 43 | 37, 512 69 | 51, 2048 219 | 108; 1 of 4096, 32/32,
-# 128 70 | 74, 256 123 | 100; 1 of 30000, 64/8, 128 108 | 91, 256 195 | 126; 8 of 2000, 32/8, 256 58 | 67, 512 102 | 107, 1024 192 | 120;
-# 2 of 400, 32/8, 256 21 | 27, 512 29 | 27.
-KV8_READ_ROWS, KV8_READ_LONG, KV8_READ_BYTES = 512, (256, 4096), 1 << 30
+# kernel attends to those, while that takes no more memory than KV8_READ_BYTES.  That kernel goes by the borders of sequences of several tokens;
+# single ones, however many heads they have, stay on the cache's bytes.  It pays where
+#   its tiles of 128 rows, up to 16 query heads of one key head each, are filled (KV8_READ_TILE rows),
+#   there is enough to do that a launch more does not count (KV8_READ_WORK: rows of queries times keys),
+#   what is read back serves enough rows of a sequence, in the mean (KV8_READ_MEAN).
+# Us of the integer products on the cache | of rows read back, sequences of one length (sequences, keys, query and key heads, rows):
+#   1 of 4096, 32/8, 64 rows 24 | 31, 128 31 | 31, 192 38 | 36, 256 46 | 37, 512 71 | 52, 2048 225 | 110
+#   1 of 30000, 64/8, 64 rows 66 | 91, 128 112 | 93, 256 203 | 129;  2 of 500, 32/8, 256 rows 17 | 29, 512 29 | 29, 1024 52 | 30
+#   8 of 2000, 32/8, 64 rows 46 | 63, 128 79 | 69, 256 135 | 81, 1024 483 | 235;  4 of 8192, 32/32, 64 rows 236 | 322, 128 445 | 327
+#   1 of 200, 8/1, 512 rows 11 | 23;  8 of 8192, 128/2, 128 rows (2 tokens: 32 rows of a tile) 68 | 127
+# Of 2022 such cases, 1 to 32 sequences of 200 to 30000 keys, the rule takes the slower way by a tenth or more in 41.
+KV8_READ_TILE, KV8_READ_WORK, KV8_READ_MEAN, KV8_READ_BYTES = 96, 5_000_000, 80, 1 << 30
 KV8_READ_SEQUENCES = 65535          # the reading kernel's grid
 KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 1024, 296, 4232
+
+
+def _kv8_reads_back(T, H, G, d, dv, n_seq, max_q, max_len):
+    """Whether reading rows back pays for ``T`` tokens of ``n_seq`` sequences of up to ``max_q`` tokens and ``max_len`` keys."""
+    work = T * H * max_len
+    return min(max_q, T) * min(H // G, 16) >= KV8_READ_TILE and work >= max(KV8_READ_WORK, KV8_READ_MEAN * n_seq * G * max_len) and \
+        n_seq <= KV8_READ_SEQUENCES and 2 * n_seq * max_len * G * (d + dv) <= KV8_READ_BYTES
 
 
 def _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):
@@ -370,9 +383,8 @@ def attention_kv8(q, words, base, length, max_len, scale, sink, alibi_slopes, wi
     (T, H, d), G, dv = q.shape, words[4], words[6]
     window = window or 0
     n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, max_q)
-    rows = max_q * (H // G)
-    if max_q > 1 and (rows >= KV8_READ_ROWS or (rows >= KV8_READ_LONG[0] and max_len >= KV8_READ_LONG[1])) and q.dtype is torch.bfloat16 and \
-            n_seq <= KV8_READ_SEQUENCES and not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4) and 2 * n_seq * max_len * G * (d + dv) <= KV8_READ_BYTES:
+    if max_q > 1 and q.dtype is torch.bfloat16 and _kv8_reads_back(T, H, G, d, dv, n_seq, max_q, max_len) and \
+            not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4):
         return _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
     out = q.new_empty((T, H, dv))
     # room for what shares cut: a call has no more CTAs than are resident, or a CTA for each key head and 16 of its query heads

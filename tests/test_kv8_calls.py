@@ -70,14 +70,32 @@ def test_single_tokens_stay_on_the_bytes_whatever_their_heads(monkeypatch):
         for max_len in (64, 5000):
             assert way(monkeypatch, 3, H, cache, max_len, None, None) == "bytes"
             assert way(monkeypatch, 3, H, cache, max_len, ints([0, 1, 2]), 1) == "bytes"
-            assert way(monkeypatch, 3, H, cache, max_len, ints([0, 2]), 2) == ("back" if 2 * H >= 512 else "bytes")
+    for T, want in ((5, "bytes"), (6, "back")):                   # 16 heads of each token fill a tile
+        assert way(monkeypatch, T, 1024, cache, 5000, ints([0, T]), T) == want
 
 
 def test_more_sequences_than_are_read_back_stay_on_the_bytes(monkeypatch):
     cache = iops.kv8_empty(64, 1, 16, 16, 16)
     for n, want in ((65535, "back"), (65536, "bytes")):
         cu = torch.arange(n + 1, dtype=torch.int32)
-        assert way(monkeypatch, n, 16, cache, 64, cu, 32) == want
+        assert way(monkeypatch, 6 * n, 16, cache, 64, 6 * cu, 6) == want
+
+
+def test_the_way_goes_by_the_work_and_by_what_a_sequence_reads(monkeypatch):
+    cache = iops.kv8_empty(64, 8, 128, 128, 16)
+
+    def of(new, H, max_len, **kw):
+        cu = ints([0] + new).cumsum(0).int()
+        return way(monkeypatch, sum(new), H, cache, max_len, cu, kw.pop("max_q", max(new)), **kw)
+    assert of([512], 32, 4096) == of([512, 1], 32, 4096) == of([64], 32, 4096) == "back"
+    assert of([512], 32, 4096, dtype=F32) == "bytes"              # the kernel takes bf16
+    assert of([23], 32, 30000) == "bytes"                         # 92 rows of a tile of 128
+    assert of([24], 32, 30000) == "back"
+    assert of([128], 8, 1000) == "bytes"                          # little to do
+    assert of([512] + [1] * 30, 32, 4096) == "bytes"              # 30 prefixes of which every row serves one token
+    assert of([512] * 16, 32, 8192) == of([512] * 32, 32, 8192) == "back"
+    assert of([512] * 33, 32, 8192) == "bytes"                    # past the memory
+    assert of([5], 32, 30000, max_q=2048) == "bytes"              # a bound that the rows do not reach
 
 
 @pytest.mark.gpu
@@ -455,6 +473,30 @@ def test_a_hybrid_model_generates_from_8_bits(device):
     assert torch.equal(out, m.generate(ids, attention_mask=mask, max_new_tokens=9, cuda_graph=False))
 
 
+# ---- rows read back, whatever the rule says ---------------------------------------------------------------------
+def read_back(monkeypatch):
+    """Calls that can be go to rows read back; the list that is given back gets an entry for each."""
+    from easyllm_b200.ops import cuda_infer as ci
+    taken, back = [], ci._attention_read_back
+    monkeypatch.setattr(ci, "_kv8_reads_back", lambda *a: True)
+    monkeypatch.setattr(ci, "_attention_read_back", lambda *a: (taken.append(1), back(*a))[1])
+    return taken
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("device", ["cuda"])
+@pytest.mark.parametrize("H,G,d,dv,new,kind", [(8, 2, 128, 128, [150, 1, 300], None), (8, 1, 64, 32, [70, 131], "sink"), (4, 4, 128, 128, [1, 530], "alibi"),
+                                               (12, 2, 48, 128, [90, 1, 1, 200], "window"), (16, 16, 16, 16, [40, 51, 1], None), (64, 2, 96, 80, [3, 2], "sink"),
+                                               (40, 1, 112, 128, [33, 5], "window")])
+def test_attention_over_rows_read_back(monkeypatch, device, H, G, d, dv, new, kind):
+    dev = _device(device)
+    taken = read_back(monkeypatch)
+    check_attention(dev, BF16, H, G, d, dv, 16, [601 + 77 * i for i in range(len(new))], new, sink=kind == "sink", alibi=kind == "alibi",
+                    window=150 if kind == "window" else None)
+    check_attention(dev, BF16, H, G, d, dv, 4, [max(new) + 3] + [1] * (len(new) - 1), new, sink=kind == "sink")
+    assert len(taken) == 2
+
+
 # ---- memory that nobody wrote ---------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("window,kind", [(None, None), (90, None), (None, "sink"), (None, "alibi")])
@@ -462,7 +504,6 @@ def test_a_hybrid_model_generates_from_8_bits(device):
 def test_rows_read_back_do_not_depend_on_what_lay_behind_them(monkeypatch, H, G, d, dv, window, kind):
     """Long continued prompts of unequal length, a sequence without rows, one whose rows see nothing, rows behind the last border: the bits
     are the same when all memory that the call allocates held NaN before."""
-    from easyllm_b200.ops import cuda_infer as ci
     dev = _device("cuda")
     cap, total, new = 1024, [700, 65, 64, 330], [150, 1, 64, 129]
     cache, plain = filled(4 * cap, G, d, dv, 16, dev)
@@ -474,9 +515,7 @@ def test_rows_read_back_do_not_depend_on_what_lay_behind_them(monkeypatch, H, G,
     q = rand(T + dead, H, d, seed=1).to(BF16).to(dev)
     sink = rand(H, seed=4).to(dev) if kind == "sink" else None
     slopes = torch.tensor([2.0 ** (-8.0 * (h + 1) / H) for h in range(H)]).to(dev) if kind == "alibi" else None
-    taken = []
-    back = ci._attention_read_back
-    monkeypatch.setattr(ci, "_attention_read_back", lambda *a: (taken.append(1), back(*a))[1])
+    taken = read_back(monkeypatch)
 
     def call():
         return iops.attention_kv8(q, cache, base, length, 720, 0.1, sink, slopes, window, cu, 160)
