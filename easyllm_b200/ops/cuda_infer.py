@@ -354,16 +354,20 @@ def kv8_read(base, length, words, max_len, dtype):
 #   1 of 30000, 64/8, 64 rows 66 | 91, 128 112 | 93, 256 203 | 129;  2 of 500, 32/8, 256 rows 17 | 29, 512 29 | 29, 1024 52 | 30
 #   8 of 2000, 32/8, 64 rows 46 | 63, 128 79 | 69, 256 135 | 81, 1024 483 | 235;  4 of 8192, 32/32, 64 rows 236 | 322, 128 445 | 327
 #   1 of 200, 8/1, 512 rows 11 | 23;  8 of 8192, 128/2, 128 rows (2 tokens: 32 rows of a tile) 68 | 127
-# Of 2022 such cases, 1 to 32 sequences of 200 to 30000 keys, the rule takes the slower way by a tenth or more in 41.
+# With a window less is to do for as much that is read back, 1 of 30000, 32/8, 2048 rows: of 64 keys 41 | 53, of 256 53 | 57, of 1024 100 | 76,
+# of 4096 244 | 143; 512 rows: of 1024 39 | 64, of 4096 78 | 80, of 16384 225 | 150.
+# Of 2022 such cases without one, 1 to 32 sequences of 200 to 30000 keys, the rule takes the slower way by a tenth or more in 41.
 KV8_READ_TILE, KV8_READ_WORK, KV8_READ_MEAN, KV8_READ_BYTES = 96, 5_000_000, 80, 1 << 30
 KV8_READ_SEQUENCES = 65535          # the reading kernel's grid
 KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 1024, 296, 4232
 
 
-def _kv8_reads_back(T, H, G, d, dv, n_seq, max_q, max_len):
-    """Whether reading rows back pays for ``T`` tokens of ``n_seq`` sequences of up to ``max_q`` tokens and ``max_len`` keys."""
-    work = T * H * max_len
-    return min(max_q, T) * min(H // G, 16) >= KV8_READ_TILE and work >= max(KV8_READ_WORK, KV8_READ_MEAN * n_seq * G * max_len) and \
+def _kv8_reads_back(T, H, G, d, dv, n_seq, max_q, max_len, window):
+    """Whether reading rows back pays for ``T`` tokens of ``n_seq`` sequences of up to ``max_q`` tokens and ``max_len`` keys, of which a
+    token sees the last ``window`` (0: all)."""
+    new = min(max_q, T)
+    work = T * H * (min(max_len, window + new - 1) if window else max_len)
+    return new * min(H // G, 16) >= KV8_READ_TILE and work >= max(KV8_READ_WORK, KV8_READ_MEAN * n_seq * G * max_len) and \
         n_seq <= KV8_READ_SEQUENCES and 2 * n_seq * max_len * G * (d + dv) <= KV8_READ_BYTES
 
 
@@ -383,7 +387,7 @@ def attention_kv8(q, words, base, length, max_len, scale, sink, alibi_slopes, wi
     (T, H, d), G, dv = q.shape, words[4], words[6]
     window = window or 0
     n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, max_q)
-    if max_q > 1 and q.dtype is torch.bfloat16 and _kv8_reads_back(T, H, G, d, dv, n_seq, max_q, max_len) and \
+    if max_q > 1 and q.dtype is torch.bfloat16 and _kv8_reads_back(T, H, G, d, dv, n_seq, max_q, max_len, window) and \
             not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4):
         return _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)
     out = q.new_empty((T, H, dv))

@@ -98,6 +98,17 @@ def test_the_way_goes_by_the_work_and_by_what_a_sequence_reads(monkeypatch):
     assert of([5], 32, 30000, max_q=2048) == "bytes"              # a bound that the rows do not reach
 
 
+def test_the_way_goes_by_what_a_window_leaves_to_do(monkeypatch):
+    """A whole prefix is not written out in 16 bits for rows that see the end of it."""
+    cache = iops.kv8_empty(64, 8, 128, 128, 16)
+
+    def of(new, max_len, window):
+        return way(monkeypatch, new, 32, cache, max_len, ints([0, new]), new, window)
+    assert of(512, 30000, 64) == of(512, 30000, 256) == of(128, 30000, 1024) == of(128, 30000, 4096) == "bytes"
+    assert of(512, 30000, 1024) == of(128, 30000, 16384) == of(512, 4096, 64) == of(2048, 30000, 64) == "back"
+    assert of(512, 30000, 1 << 40) == of(512, 30000, None) == "back"
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("device", ["cuda"])
 def test_attention_of_more_sequences_than_are_read_back(device):
