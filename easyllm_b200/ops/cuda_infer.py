@@ -359,6 +359,7 @@ def kv8_read(base, length, words, max_len, dtype):
 # Of 2022 such cases without one, 1 to 32 sequences of 200 to 30000 keys, the rule takes the slower way by a tenth or more in 41.
 KV8_READ_TILE, KV8_READ_WORK, KV8_READ_MEAN, KV8_READ_BYTES = 96, 5_000_000, 80, 1 << 30
 KV8_READ_SEQUENCES = 65535          # the reading kernel's grid
+KV8_LONGEST = 0x3fffffff            # rows of a sequence that the kernels count with: a window of more hides nothing
 KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 1024, 296, 4232
 
 
@@ -385,7 +386,7 @@ def _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slo
 @_on_device
 def attention_kv8(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):
     (T, H, d), G, dv = q.shape, words[4], words[6]
-    window = window or 0
+    window = min(window or 0, KV8_LONGEST)
     n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, max_q)
     if max_q > 1 and q.dtype is torch.bfloat16 and _kv8_reads_back(T, H, G, d, dv, n_seq, max_q, max_len, window) and \
             not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4):

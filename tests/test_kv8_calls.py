@@ -109,6 +109,21 @@ def test_the_way_goes_by_what_a_window_leaves_to_do(monkeypatch):
     assert of(512, 30000, 1 << 40) == of(512, 30000, None) == "back"
 
 
+@pytest.mark.parametrize("window", [(1 << 31) + 3, (1 << 32) + 5, 1 << 70])
+def test_windows_past_32_bits_are_not_cut_to_them(monkeypatch, window):
+    """Both ways get a window that hides nothing, in the words that they have for it."""
+    from easyllm_b200.ops import cuda_infer as ci
+    cache, seen = iops.kv8_empty(64, 8, 128, 128, 16), []
+    monkeypatch.setattr(ci, "_attention_read_back", lambda q, words, base, length, max_len, scale, sink, slopes, window, *a: seen.append(window))
+    monkeypatch.setattr(ci, "_kv8_call", lambda name, label, n, *words: seen.append(ci._KV8_CALLS[name](*words) and words[24]))
+    monkeypatch.setattr(ci, "_err_word", lambda device: 0)
+    for new, max_len in ((512, 4096), (2, 64)):
+        places = ints([0] * new)
+        ci.attention_kv8.__wrapped__(torch.empty(new, 32, 128, dtype=BF16), iops._kv8_check(cache, places), places, places, max_len, 1.0, None, None,
+                                     window, ints([0, new]), new)
+    assert len(seen) == 2 and all(4096 <= w < 1 << 31 for w in seen)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("device", ["cuda"])
 def test_attention_of_more_sequences_than_are_read_back(device):
