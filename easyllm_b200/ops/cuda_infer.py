@@ -330,7 +330,7 @@ def _is_bf(dtype):
 @_on_device
 def kv8_append(k, v, words, base, length, cu_seqlens, max_new):
     _kv8_call("ell_kv8_append", "kv8_append", 1, *words, k.data_ptr(), v.data_ptr(), base.data_ptr(), length.data_ptr(), cu_seqlens.data_ptr(),
-              k.shape[0], cu_seqlens.numel() - 1, max_new, _packed(k, "k"), _packed(v, "v"), _is_bf(k.dtype), _err_word(k.device))
+              k.shape[0], cu_seqlens.numel() - 1, min(max_new, k.shape[0]), _packed(k, "k"), _packed(v, "v"), _is_bf(k.dtype), _err_word(k.device))
 
 
 @_on_device
@@ -366,9 +366,8 @@ KV8_UNCUT, KV8_CTAS, KV8_CTA_FLOATS = 1024, 296, 4232
 def _kv8_reads_back(T, H, G, d, dv, n_seq, max_q, max_len, window):
     """Whether reading rows back pays for ``T`` tokens of ``n_seq`` sequences of up to ``max_q`` tokens and ``max_len`` keys, of which a
     token sees the last ``window`` (0: all)."""
-    new = min(max_q, T)
-    work = T * H * (min(max_len, window + new - 1) if window else max_len)
-    return new * min(H // G, 16) >= KV8_READ_TILE and work >= max(KV8_READ_WORK, KV8_READ_MEAN * n_seq * G * max_len) and \
+    work = T * H * (min(max_len, window + max_q - 1) if window else max_len)
+    return max_q * min(H // G, 16) >= KV8_READ_TILE and work >= max(KV8_READ_WORK, KV8_READ_MEAN * n_seq * G * max_len) and \
         n_seq <= KV8_READ_SEQUENCES and 2 * n_seq * max_len * G * (d + dv) <= KV8_READ_BYTES
 
 
@@ -387,7 +386,9 @@ def _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slo
 def attention_kv8(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q):
     (T, H, d), G, dv = q.shape, words[4], words[6]
     window = min(window or 0, KV8_LONGEST)
-    n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, max_q)
+    # bounds may be far off: a sequence has no more tokens than there are rows, and is no longer than the cache
+    n_seq, max_q = (0, 1) if cu_seqlens is None else (cu_seqlens.numel() - 1, min(max_q, T))
+    max_len = min(max_len, words[8])
     if max_q > 1 and q.dtype is torch.bfloat16 and _kv8_reads_back(T, H, G, d, dv, n_seq, max_q, max_len, window) and \
             not ((d | dv) % 16 or (q.data_ptr() | 2 * q.stride(0)) % 4):
         return _attention_read_back(q, words, base, length, max_len, scale, sink, alibi_slopes, window, cu_seqlens, max_q)

@@ -57,7 +57,8 @@ def way(monkeypatch, T, H, cache, max_len, cu_seqlens, max_q, window=None, dtype
     monkeypatch.setattr(ci, "_err_word", lambda device: 0)
     places = ints([0] * T)
     q = torch.empty(T, H, cache.dim, dtype=dtype)
-    ci.attention_kv8.__wrapped__(q, iops._kv8_check(cache, places), places, places, max_len, 1.0, None, None, window, cu_seqlens, max_q)
+    words = iops._kv8_check(cache, places)[:-1] + (1 << 30,)      # as of a cache with any number of rows
+    ci.attention_kv8.__wrapped__(q, words, places, places, max_len, 1.0, None, None, window, cu_seqlens, max_q)
     assert len(taken) == 1
     return taken[0]
 
@@ -119,8 +120,8 @@ def test_windows_past_32_bits_are_not_cut_to_them(monkeypatch, window):
     monkeypatch.setattr(ci, "_err_word", lambda device: 0)
     for new, max_len in ((512, 4096), (2, 64)):
         places = ints([0] * new)
-        ci.attention_kv8.__wrapped__(torch.empty(new, 32, 128, dtype=BF16), iops._kv8_check(cache, places), places, places, max_len, 1.0, None, None,
-                                     window, ints([0, new]), new)
+        ci.attention_kv8.__wrapped__(torch.empty(new, 32, 128, dtype=BF16), iops._kv8_check(cache, places)[:-1] + (1 << 30,), places, places, max_len,
+                                     1.0, None, None, window, ints([0, new]), new)
     assert len(seen) == 2 and all(4096 <= w < 1 << 31 for w in seen)
 
 
@@ -279,6 +280,28 @@ def test_lengths_beyond_their_bound_are_reported(dtype, max_len, total, new):
                 cuda.check_err_flag()
         for r in range(new):
             near(got[r], *plain_attention(q[r], *(p.values(0, total - new + 1 + r) for p in plain), 0.2))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("block", [1, 16])
+def test_bounds_that_are_far_off(device, dtype, block):
+    """``max_seqlen``, ``max_q`` and ``max_len`` say "at most": of a call's rows, or of the cache, there are never more."""
+    dev = _device(device)
+    cache, plain = filled(256, 2, 32, 16, block, dev)
+    T, far = 9, 1 << 40
+    k, v, q = (rand(T, n, w, seed=n + w).to(dtype).to(dev) for n, w in ((2, 32), (2, 16), (4, 32)))
+    meta = step([5, 4], [40, 0], [1, 0], 128, dev)
+    iops.kv8_append(cache, k, v, dict(meta, max_seqlen=far))
+    for p, x in zip(plain, (k, v)):
+        p.append(128, 40, x[:5])
+        p.append(0, 0, x[5:])
+    for x, p in zip(iops.kv8_read(cache, ints([0], dev), ints([256], dev), 256, F32), plain):
+        assert torch.equal(x[0].double().cpu(), p.values(0, 256))
+    for kw in (dict(cu_seqlens=meta["cu_seqlens"], max_q=far), {}):
+        got = iops.attention_kv8(q, cache, meta["kv_base"], meta["kv_len"], far, 0.2, **kw)
+        for r, (b, n) in enumerate(zip(meta["kv_base"].tolist(), meta["kv_len"].tolist())):
+            near(got[r], *plain_attention(q[r], *(p.values(b, n) for p in plain), 0.2))
 
 
 @pytest.mark.parametrize("device", DEVICES)
