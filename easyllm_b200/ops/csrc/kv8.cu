@@ -249,9 +249,9 @@ __device__ __forceinline__ void k8_store_values(T* o, const uint32_t* w, float s
 // row_base[r] becomes the place of a query row's keys in ko, row_base[rows + r] its length, max_len at most; both are 0 for rows behind the
 // last sequence.  A thread keeps its place in a row, V
 // elements, and takes positions, eight of which are under way together.  Bound by memory: 8 prefixes of up to 4096 rows, 8 heads of 128 (37 MB
-// in, 134 MB out, zeros among them) 31 us, 5.5 TB/s.  With a division for every eight values it took 48 us, with conversions of the integers
-// 39, with 16 values a thread, whose stores leave every other 16 bytes to the next one, 134.  One prompt of 4096 rows of 32 heads 18.5 us; 27 where
-// a CTA took four positions of whole rows.
+// in, 134 MB out, zeros among them) 30 us among others, 5.7 TB/s, 35 alone with a cold L2.  With a division for every eight values it took
+// 48 us, with conversions of the integers 39, with 16 values a thread, whose stores leave every other 16 bytes to the next one, 134.  One
+// prompt of 4096 rows of 32 heads 18.5 us; 27 where a CTA took four positions of whole rows.
 template <typename T, int V>
 __global__ void __launch_bounds__(256, 4)
 kv8_read_kernel(const Kv8Cache c, T* __restrict__ ko, T* __restrict__ vo, const int* __restrict__ base, const int* __restrict__ len,
@@ -328,7 +328,8 @@ kv8_clear_kernel(__nv_bfloat16* __restrict__ out, const int* __restrict__ len, c
 // All products are integer products of the tensor cores (mma.sync m16n8k32), of the cache's bytes as they are: nothing is converted on
 // the way, 23 bytes a clock and SM at the memory's rate.  A query row becomes integers of 23 bits, in units of 2^-21 of its largest
 // element's power of two, a weight times its value's scale integers of 23 bits of the largest of 64 of them; each is cut into three bytes,
-// which are rows of the left operand, and the three 32-bit sums, exact, join in fp32.  So scores and sums are as good as fp32 ones.
+// which are rows of the left operand, and the three 32-bit sums, exact, join in fp32.  So scores and sums are as good as fp32 ones where a row's
+// elements are of one size (4e-7 to 8e-7 off 64 bits in the norm, as fp32 sums are); one that is 2^k below its row's largest has k bits less.
 //   rows    groups of 8 (token, head): row r of the operand is the low byte of row r, row r + 8 its middle byte; the high bytes take a
 //           second product, whose upper half is empty or another group's
 //   keys    lane (g = lane / 4, c = lane % 4) holds bytes 32 c .. 32 c + 31 of key g of 8: the columns may come in any order, the queries' do so too
@@ -337,10 +338,11 @@ kv8_clear_kernel(__nv_bfloat16* __restrict__ out, const int* __restrict__ len, c
 //   rings   rows of 128 bytes with TMA's 128-byte swizzle: neither access meets a bank conflict
 // Bound by memory where sequences are long, by what begins and ends a call (3 us until the first copy, 5 for the join) where they are short.
 // Bytes of the cache a second, and us beside those of attention over the same cache in 16 bits: 64 sequences of up to 8192 keys, 32 heads
-// on 8, 5.6 TB/s, 99 (216); 24 of up to 4096, 32 on 32, 5.4, 78 (149); one of 131071, 64 on 8, 4.7, 58 (92); 6 of up to 1900 with 5 tokens
-// each, 40 on 40, 2.5, 27 (52); one of 203 keys 6.3 us (8.2).  Steps, us of the first two: a warp a row on the fp32 units 8398 and 4193;
-// integer products with 32 keys a step, a CTA an item 153 and 103; equal shares, 64 keys a step 119 and 100; found and joined with fewer
-// barriers 110 and 91; two CTAs an SM with three stages in place of three with two 105 and 86; items' beginnings counted 103 and 85.
+// on 8, 5.3 to 5.6 TB/s by the GPU, 98 to 105 (216); 24 of up to 4096, 32 on 32, 4.9 to 5.4, 78 to 86 (149); one of 131071, 64 on 8, 4.7, 58
+// (92); 6 of up to 1900 with 5 tokens each, 40 on 40, 2.5, 27 (52); one of 203 keys 5.5 (5.6) in a chain of calls, 10.2 (10.2) alone with a
+// cold L2: there the cache's size counts for nothing.  Two groups of rows (NB = 2) take 255 registers and spill 80 bytes.
+// Steps, us of the first two: a warp a row on the fp32 units 8398 and 4193; integer products with 32 keys a step, a CTA an item 153 and 103;
+// equal shares, 64 keys a step 119 and 100; found and joined with fewer barriers 110 and 91; two CTAs an SM with three stages in place of three with two 105 and 86; items' beginnings counted 103 and 85.
 constexpr int kK8Threads = 128, kK8Keys = 64, kK8Stage = kK8Keys * 128;       // a stage: keys, or values
 // Stages of a warp and CTAs an SM, which are to fit a split of 196 KB with the system's 1 KB each (112 bytes more take 228 KB, which later
 // kernels find their L1 cut down by).
@@ -1171,7 +1173,7 @@ ELL_API int ell_kv8_read(const Kv8ReadCall* call, cudaStream_t stream) {
   if (x.n <= 0 || x.max_len <= 0) return 0;
   if (!k8_cache(x.c, c) || x.n > 65535 || x.max_len > 0x3fffffff || (x.cu != nullptr && x.n * x.max_len > 0x7fffffff)) return -2;
   const int vec = c.d % 8 == 0 && c.dv % 8 == 0 ? 8 : 1;
-  // a thread takes eight positions (with sixteen or thirty-two the 31 us beside kv8_read_kernel become 32 and 35)
+  // a thread takes eight positions (the prefixes beside kv8_read_kernel took 31 us so, 32 with sixteen, 35 with thirty-two)
   const int per = c.G * (c.d + c.dv) / vec, beside = std::max(1, 256 / per), z = (beside * per + 255) / 256, chunk = 8 * beside;
   if (z > 65535) return -2;
   const dim3 grid((unsigned)((x.max_len + chunk - 1) / chunk), (unsigned)x.n, (unsigned)z);

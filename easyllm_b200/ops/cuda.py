@@ -103,7 +103,8 @@ def check_err_flag():
                           "17 its work items; 14 latent attention over cached rows, 18 attention over cached rows; 21-24 the attention's "
                           "backward pass, 21 also the cross-entropy exchange; "
                           "31 a token id outside the embedding table; 32 a position outside the rotary tables; "
-                          "41 a scan over chunks; 51 a sequence outside an 8-bit cache, or one that starts inside a block of it, 52 attention over one; "
+                          "41 a scan over chunks; 51 a sequence outside an 8-bit cache, one that starts inside a block of it, or one beyond "
+                          "the call's bounds, 52 attention over such a cache; "
                           "6 / 16 a tile index outside a fused kernel's buffers)")
 
 

@@ -247,7 +247,7 @@ class KV8(NamedTuple):
     128).  A value is ``int8 * scale``.  Scales are powers of two, the least of which 127 times is the block's largest magnitude or more (at most
     2^121: larger values become 127 times that), so that nothing but the rounding to 8 bits is ever lost: values are exact in bf16 and fp32,
     and in a block that rows join one by one they are off by less than one scale.  Where a block got a value that is not finite, it reads as
-    NaN."""
+    NaN.  The parts are contiguous, and k and v start on a 16-byte boundary."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
@@ -321,9 +321,10 @@ def kv8_read(cache, kv_base, kv_len, max_len, dtype=torch.bfloat16):
 
 def attention_kv8(q, cache, kv_base, kv_len, max_len, scale, sink=None, alibi_slopes=None, window=None, cu_seqlens=None, max_q=None):
     """``attention_rows`` over an 8-bit cache: row t of q ``[T, H, dim]`` attends to the cache rows ``kv_base[t]`` .. ``kv_base[t] + kv_len[t]``
-    and sits at the last of them.  ``max_len`` bounds ``kv_len`` (on a GPU a longer one sets the error word).  ``cu_seqlens`` (with ``max_q``, a bound of their lengths): the rows between two
-    borders are consecutive tokens of one sequence, so they can share its keys.  Rows with nothing to see (``kv_len`` 0, or behind the last
-    border) are zero."""
+    and sits at the last of them.  ``max_len`` bounds ``kv_len`` (on a GPU a longer one sets the error word).  ``cu_seqlens`` (with ``max_q``, a
+    bound of their lengths): the rows between two borders are consecutive tokens of one sequence, so they can share its keys.  Rows with nothing to see (``kv_len`` 0, or behind the last
+    border) are zero.  The kernels hold a query head as integers of 23 bits of its largest element, and 64 weights times their values' scales as
+    such of the largest of them: in fp32 too, an element that is 2^k times smaller than the largest beside it has k bits less."""
     no_grad_check(q)
     ints = (kv_base, kv_len) if cu_seqlens is None else (kv_base, kv_len, cu_seqlens)
     words = _kv8_check(cache, *ints)
