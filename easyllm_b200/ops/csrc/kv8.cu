@@ -751,10 +751,10 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   chain_enter();
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, gr = lane >> 2, c = lane & 3;
   const int n_x = a.cu != nullptr ? a.n_seq * a.tiles : a.n, hs = k8_groups(a.H, a.c.G), rep = a.H / a.c.G, groups = hs / a.c.G;
-  if (a.cu != nullptr && blockIdx.x == 0) {            // rows behind the last sequence
+  if (a.cu != nullptr) {                               // rows behind the last sequence, by all CTAs (by one, 4096 of 32 heads took 550 us)
     T* out = reinterpret_cast<T*>(a.out);
-    const long long per = (long long)a.H * a.c.dv;
-    for (long long i = min(max(a.cu[a.n_seq], 0), a.n) * per + threadIdx.x; i < a.n * per; i += kK8Threads) out[i] = from_f<T>(0.f);
+    const long long per = (long long)a.H * a.c.dv, first = (long long)blockIdx.x * kK8Threads + threadIdx.x;
+    for (long long i = min(max(a.cu[a.n_seq], 0), a.n) * per + first; i < a.n * per; i += (long long)gridDim.x * kK8Threads) out[i] = from_f<T>(0.f);
   }
   const int hg = blockIdx.x % hs, share = blockIdx.x / hs, g = hg / groups, h0 = g * rep + hg % groups * kK8Heads;
   const int nh = min(kK8Heads, (g + 1) * rep - h0);

@@ -589,3 +589,29 @@ def test_rows_read_back_do_not_depend_on_what_lay_behind_them(monkeypatch, H, G,
             low = max(0, end - window) if window else 0
             near(got[r + j], *plain_attention(q[r + j], *(p.values(s * cap + low, end - low) for p in plain), 0.1, sink, slopes))
         r += n
+
+
+# ---- padded batches ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("G,dv,longest,pad", [(2, 64, 90, 1000), (1, 7, 90, 1000), (2, 12, 1500, 333), (1, 9, 1500, 1), (4, 16, 1500, 2000)])
+def test_rows_of_a_padded_batch_are_zero(device, dtype, G, dv, longest, pad):
+    """Few tokens in front of many rows behind the last border: every one of those is zero, in memory that held NaN, and no other is."""
+    dev = _device(device)
+    cap, H, d = 1536, 4, 32
+    cache, plain = filled(2 * cap, G, d, dv, 16, dev)
+    total, new = [longest, 40], [3, 2]
+    meta = step(new, [t - c for t, c in zip(total, new)], [1, 0], cap, dev)
+    T = sum(new)
+    q = rand(T + pad, H, d, seed=1).to(dtype).to(dev)
+    base, length = (torch.cat((meta[n], ints([-1] * pad, dev))) for n in ("kv_base", "kv_len"))
+    for _ in range(3):
+        held = [torch.full((T + pad, H, dv), float("nan"), dtype=dtype, device=dev) for _ in range(3)]
+        del held                                                  # the allocator hands this memory out again
+        got = iops.attention_kv8(q, cache, base, length, longest, 0.2, cu_seqlens=meta["cu_seqlens"], max_q=3)
+        assert not bool(got[T:].any())
+        r = 0
+        for t, c, s in zip(total, new, (1, 0)):
+            for j in range(c):
+                near(got[r], *plain_attention(q[r], *(p.values(s * cap, t - c + j + 1) for p in plain), 0.2))
+                r += 1
