@@ -247,8 +247,8 @@ __device__ __forceinline__ void k8_store_values(T* o, const uint32_t* w, float s
 // ko [n, max_len, G, d], vo [n, max_len, G, dv].  cu null: rows base[i] .. base[i] + len[i] - 1 of the cache, then zeros.  Otherwise sequence i has
 // the query rows cu[i] .. cu[i + 1] - 1 with base and len of their own: its rows are those that its last one sees, nothing is written behind them,
 // row_base[r] becomes the place of a query row's keys in ko, row_base[rows + r] its length, max_len at most; both are 0 for rows behind the
-// last sequence.  A thread keeps its place in a row, V
-// elements, and takes positions, eight of which are under way together.  Bound by memory: 8 prefixes of up to 4096 rows, 8 heads of 128 (37 MB
+// last sequence.  A thread keeps its place in a row, V elements, and takes positions, eight of which are under way together.
+// Bound by memory: 8 prefixes of up to 4096 rows, 8 heads of 128 (37 MB
 // in, 134 MB out, zeros among them) 30 us among others, 5.7 TB/s, 35 alone with a cold L2.  With a division for every eight values it took
 // 48 us, with conversions of the integers 39, with 16 values a thread, whose stores leave every other 16 bytes to the next one, 134.  One
 // prompt of 4096 rows of 32 heads 18.5 us; 27 where a CTA took four positions of whole rows.
@@ -342,7 +342,8 @@ kv8_clear_kernel(__nv_bfloat16* __restrict__ out, const int* __restrict__ len, c
 // (92); 6 of up to 1900 with 5 tokens each, 40 on 40, 2.5, 27 (52); one of 203 keys 5.5 (5.6) in a chain of calls, 10.2 (10.2) alone with a
 // cold L2: there the cache's size counts for nothing.  Two groups of rows (NB = 2) take 255 registers and spill 80 bytes.
 // Steps, us of the first two: a warp a row on the fp32 units 8398 and 4193; integer products with 32 keys a step, a CTA an item 153 and 103;
-// equal shares, 64 keys a step 119 and 100; found and joined with fewer barriers 110 and 91; two CTAs an SM with three stages in place of three with two 105 and 86; items' beginnings counted 103 and 85.
+// equal shares, 64 keys a step 119 and 100; found and joined with fewer barriers 110 and 91; two CTAs an SM with three stages in place of
+// three with two 105 and 86; items' beginnings counted 103 and 85.
 constexpr int kK8Threads = 128, kK8Keys = 64, kK8Stage = kK8Keys * 128;       // a stage: keys, or values
 // Stages of a warp and CTAs an SM, which are to fit a split of 196 KB with the system's 1 KB each (112 bytes more take 228 KB, which later
 // kernels find their L1 cut down by).

@@ -322,8 +322,8 @@ def kv8_read(cache, kv_base, kv_len, max_len, dtype=torch.bfloat16):
 def attention_kv8(q, cache, kv_base, kv_len, max_len, scale, sink=None, alibi_slopes=None, window=None, cu_seqlens=None, max_q=None):
     """``attention_rows`` over an 8-bit cache: row t of q ``[T, H, dim]`` attends to the cache rows ``kv_base[t]`` .. ``kv_base[t] + kv_len[t]``
     and sits at the last of them.  ``max_len`` bounds ``kv_len`` (on a GPU a longer one sets the error word).  ``cu_seqlens`` (with ``max_q``, a
-    bound of their lengths): the rows between two borders are consecutive tokens of one sequence, so they can share its keys.  Rows with nothing to see (``kv_len`` 0, or behind the last
-    border) are zero.  The kernels hold a query head as integers of 23 bits of its largest element, and 64 weights times their values' scales as
+    bound of their lengths): the rows between two borders are consecutive tokens of one sequence, so they can share its keys.  Rows with
+    nothing to see (``kv_len`` 0, or behind the last border) are zero.  The kernels hold a query head as integers of 23 bits of its largest element, and 64 weights times their values' scales as
     such of the largest of them: in fp32 too, an element that is 2^k times smaller than the largest beside it has k bits less."""
     no_grad_check(q)
     ints = (kv_base, kv_len) if cu_seqlens is None else (kv_base, kv_len, cu_seqlens)
