@@ -546,6 +546,20 @@ def test_attention_over_rows_read_back(monkeypatch, device, H, G, d, dv, new, ki
     assert len(taken) == 2
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("device", ["cuda"])
+def test_rows_read_back_keep_what_is_not_finite_and_what_sees_nothing(monkeypatch, device):
+    """The cases of such rows, and of rows past two gigabytes, by this way."""
+    import test_kv8 as cases
+    taken = read_back(monkeypatch)
+    cases.test_long_prompts_beside_rows_that_see_nothing(device, BF16)
+    cases.test_what_is_not_finite_reaches_the_rows_that_see_it(device, BF16, 60)
+    cases.test_rows_that_see_nothing_are_zero(device, BF16, True)
+    cases.test_rows_past_two_gigabytes()
+    cases.test_steps_of_a_conversation(device, BF16)
+    assert len(taken) >= 5
+
+
 # ---- memory that nobody wrote ---------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("window,kind", [(None, None), (90, None), (None, "sink"), (None, "alibi")])
@@ -615,3 +629,57 @@ def test_rows_of_a_padded_batch_are_zero(device, dtype, G, dv, longest, pad):
             for j in range(c):
                 near(got[r], *plain_attention(q[r], *(p.values(s * cap, t - c + j + 1) for p in plain), 0.2))
                 r += 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("back", [False, True])
+def test_a_captured_step_takes_any_batch_that_fits_it(monkeypatch, back):
+    """A step of a fixed number of rows and sequences, captured once: its replays write and attend for whatever tokens the borders name then,
+    the rows behind them are zero, and the bits are those of eager calls."""
+    from easyllm_b200.ops import cuda
+    dev = _device("cuda")
+    G, H, d, cap, T, slots = 2, 8, 64, 1536, 300, 3
+    taken = read_back(monkeypatch) if back else []
+    cache, plain = filled(slots * cap, G, d, d, 16, dev)
+    had, before = [t.clone() for t in cache[:4]], [(p.q.clone(), p.s.clone()) for p in plain]
+    k, v, q = (torch.zeros(T, n, d, dtype=BF16, device=dev) for n in (G, G, H))
+    meta = {"kv_base": ints([0] * T, dev), "kv_len": ints([0] * T, dev), "cu_seqlens": ints([0] * (slots + 1), dev), "max_seqlen": 200}
+
+    def run():
+        iops.kv8_append(cache, k, v, meta)
+        return iops.attention_kv8(q, cache, meta["kv_base"], meta["kv_len"], cap, 0.15, cu_seqlens=meta["cu_seqlens"], max_q=200)
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for i, (counts, start, order) in enumerate([([200, 1, 99], [0, 1300, 40], [2, 0, 1]), ([1, 1, 1], [1535, 0, 17], [0, 1, 2]), ([0, 0, 0], [0, 0, 0], [0, 1, 2]),
+                                                ([0, 120, 2], [0, 1400, 999], [1, 2, 0]), ([100, 100, 100], [5, 600, 1234], [0, 2, 1])]):
+        m = step(counts, start, order, cap, dev)
+        n = sum(counts)
+        for name, pad in (("kv_base", -5), ("kv_len", 1 << 30)):  # rows behind the last border say anything
+            meta[name].fill_(pad)
+            meta[name][:n] = m[name]
+        meta["cu_seqlens"].copy_(m["cu_seqlens"])
+        for j, t in enumerate((k, v, q)):
+            t.copy_(rand(*t.shape, seed=10 * i + j).to(BF16))
+        results = []
+        for call in (graph.replay, run):
+            for t, h in zip(cache[:4], had):
+                t.copy_(h)
+            got = call()
+            results.append([t.clone() for t in cache[:4]] + [(out if got is None else got).clone()])
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+        got = results[0][-1]
+        assert not bool(got[n:].any())
+        r = 0
+        for c, p0, s in zip(counts, start, order):
+            for p, (q0, s0), x in zip(plain, before, (k, v)):     # each step starts from the same cache
+                p.q.copy_(q0), p.s.copy_(s0)
+                if c:
+                    p.append(s * cap, p0, x[r:r + c])
+            for j in sorted({0, c // 2, c - 1} if c else ()):
+                near(got[r + j], *plain_attention(q[r + j], *(p.values(s * cap, p0 + j + 1) for p in plain), 0.15))
+            r += c
+    cuda.check_err_flag()
+    assert not back or len(taken) >= 7
